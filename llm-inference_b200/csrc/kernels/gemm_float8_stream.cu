@@ -1,0 +1,450 @@
+// Product of 8-bit rows for few tokens: the weights stream past the tensor cores once, K split inside thread-block clusters.
+//   y[m][n] = act((sum_k x[m][k] w[n][k]) xs[m] ws[n] + bias[n]) + residual[m][n],  or act(gate) * up over pairs of W's rows.
+//
+// W is the wide operand: a block owns 128 rows of W (the MMA's M) and a tile of up to 256 tokens (its N, a multiple of 16). One thread fills a ring
+// of stages by TMA (128 rows x 128 bytes of W, tokens x 128 bytes of X, 128-byte swizzle), one issues `tcgen05.mma` (kind::f8f6f4, 32 k an
+// instruction) into TMEM, four warps read the sums back, a lane per row of W. Where W has too few rows to give every SM work, the blocks of a
+// cluster share rows and split K: each pushes its partial sums into the shared memory of the member that finishes those rows, the cluster meets,
+// and the owners add in member order, so a sum does not depend on timing. With up to 16 tokens the inboxes lie behind the ring and the
+// cluster meets once; with more they take the ring's place, so it meets before the push too (stores into a neighbour's memory need no answer, loads
+// out of it wait for one).
+//
+// 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as TMEM goes, added up as they are read.
+//
+// The first stages' weights are asked for before the kernel in front has ended where the caller says that nothing still writes them; TMEM is
+// taken only after it has (a block that held TMEM while a kernel in front still wanted some could keep both waiting). A block takes no larger a
+// share of an SM's TMEM than of its shared memory, so a resident block never waits for another's. Every wait is bounded: a block that gives
+// up sets the timeout bit, waits for its copies in flight, frees its TMEM and leaves.
+#include <mutex>
+#include <vector>
+
+#include "float8.cuh"
+
+namespace float8 {
+namespace {
+
+constexpr int kThreads = 192;      // warp 0: TMA, warp 1: MMA, warps 2-5: sums
+constexpr int kMaxStages = 12;
+constexpr int kMaxMembers = 16;
+constexpr int kEarlyTokens = 16;   // up to this many (padded) tokens the inboxes lie behind the ring
+constexpr int kMaxTokens = 256;    // a block's
+
+struct StreamParams {
+  Epilogue e;
+  int* err;
+  int K;
+  int stages;
+  int tile;          // tokens of a block, a multiple of 16
+  int chain_blocks;  // k-blocks per accumulator
+  int tmem_cols;
+  int w_constant;
+};
+
+// Rows of a block that one member of a cluster finishes; gate and up stay together.
+__host__ __device__ constexpr int slice_rows(int members) { return (((kRowsW + members - 1) / members) + 1) & ~1; }
+
+__device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// A form carries no code that it does not take: a block runs its epilogue once, from a cold instruction cache (measured in gemm_tcgen05.cu).
+template <int KIND, typename T, bool CLUSTERED>
+__global__ void __launch_bounds__(kThreads)
+float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const StreamParams p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t w_bytes = kRowsW * kBlockK;
+  const uint32_t x_bytes = static_cast<uint32_t>(p.tile) * kBlockK;
+  const uint32_t stage_bytes = w_bytes + ((x_bytes + 1023u) & ~1023u);
+  unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full_bar[kMaxStages];
+  __shared__ __align__(8) uint64_t empty_bar[kMaxStages];
+  __shared__ __align__(8) uint64_t accum_bar;
+  __shared__ uint32_t tmem_base_shared;
+  __shared__ float x_scales[kMaxTokens];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stages = p.stages;
+  const int n0 = blockIdx.x * kRowsW;
+  const int m0 = blockIdx.z * p.tile;
+  const int members = gridDim.y, rank = blockIdx.y;
+  const int k_blocks = (p.K + kBlockK - 1) / kBlockK;
+  const int kb_begin = static_cast<int>(static_cast<int64_t>(k_blocks) * rank / members);
+  const int num_kb = static_cast<int>(static_cast<int64_t>(k_blocks) * (rank + 1) / members) - kb_begin;  // at least one: members <= k_blocks
+  const int first = min(num_kb, stages);
+
+  auto load_w = [&](int i) { tma_load_2d(tiles + (i % stages) * stage_bytes, &w_map, &full_bar[i % stages], (kb_begin + i) * kBlockK, n0); };
+  auto load_x = [&](int i) { tma_load_2d(tiles + (i % stages) * stage_bytes + w_bytes, &x_map, &full_bar[i % stages], (kb_begin + i) * kBlockK, m0); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&accum_bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // The thread that made the barriers also loads: the first weights are on their way before the block has met.
+    if (!p.w_constant) wait_for_predecessor();
+    for (int i = 0; i < first; ++i) {
+      mbar_expect_tx(&full_bar[i], w_bytes + x_bytes);
+      load_w(i);
+    }
+    wait_for_predecessor();
+    for (int i = 0; i < first; ++i) load_x(i);
+  }
+  wait_for_predecessor();
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_shared)),
+                 "r"(static_cast<uint32_t>(p.tmem_cols))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp >= 2) {
+    for (int i = threadIdx.x - 64; i < p.tile; i += 128) x_scales[i] = m0 + i < p.e.M ? p.e.x_scale[m0 + i] : 0.f;
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  let_successor_start();
+  const uint32_t tmem_base = tmem_base_shared;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int sent = first;
+      for (; sent < num_kb; ++sent) {
+        const int s = sent % stages;
+        if (!mbar_wait(&empty_bar[s], ((sent / stages) - 1) & 1)) {
+          atomicOr(p.err, ERRBIT_TIMEOUT);
+          for (int i = max(0, sent - stages); i < sent; ++i) mbar_wait(&full_bar[i % stages], (i / stages) & 1);  // copies in flight
+          break;
+        }
+        mbar_expect_tx(&full_bar[s], w_bytes + x_bytes);
+        load_w(sent);
+        load_x(sent);
+      }
+    }
+  } else if (warp == 1) {
+    // The whole warp walks the loop and one elected lane issues, so that descriptors stay in uniform registers.
+    const bool leader = elect_one();
+    const uint32_t idesc = instr_desc(kRowsW, p.tile);
+    const uint64_t a_first = smem_desc(smem_addr(tiles)), b_first = smem_desc(smem_addr(tiles) + w_bytes);
+    int s = 0, phase = 0, link = 0;
+    uint32_t accumulator = tmem_base;
+    for (int i = 0; i < num_kb; ++i) {
+      if (!mbar_wait(&full_bar[s], phase)) {
+        if (leader) atomicOr(p.err, ERRBIT_TIMEOUT);
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t stage_units = static_cast<uint64_t>(s) * (stage_bytes >> 4);
+#pragma unroll
+      for (int k = 0; k < kBlockK / kMmaK; ++k) {
+        const uint64_t step = stage_units + static_cast<uint64_t>(k * (kMmaK >> 4));
+        if (leader) umma(accumulator, a_first + step, b_first + step, idesc, link > 0 || k > 0);
+      }
+      if (leader) umma_commit(&empty_bar[s]);
+      __syncwarp();
+      if (++s == stages) s = 0, phase ^= 1;
+      if (++link == p.chain_blocks) link = 0, accumulator += p.tile;
+    }
+    if (leader) umma_commit(&accum_bar);
+  }
+  __syncwarp();
+
+  const int slice = slice_rows(members);
+  const bool early = p.tile <= kEarlyTokens;
+  // [members][tokens][slice] partial sums, behind the ring or (once every member is done with its products) in its place.
+  float* inbox = reinterpret_cast<float*>(tiles + (early ? static_cast<size_t>(stages) * stage_bytes : 0));
+  const int tokens = min(p.tile, p.e.M - m0);
+  const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31 belong to this warp
+  const int row = quarter * 32 + lane;
+  if (warp >= 2) {
+    const int n = n0 + row;
+    float ws = 0.f, b = 0.f;
+    if (!CLUSTERED && n < p.e.N) {
+      ws = p.e.w_scale[n];
+      if (p.e.bias != nullptr) b = p.e.bias[n];
+    }
+    const bool have = mbar_wait(&accum_bar, 0);
+    if (!have && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if constexpr (!CLUSTERED) {
+      const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
+      for (int c0 = 0; have && c0 < tokens; c0 += 16) {
+        float v[16];
+        const uint32_t at = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
+        tmem_load_16(at, v);
+        for (int c = 1; c < chains; ++c) {
+          float more[16];
+          tmem_load_16(at + c * p.tile, more);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] += more[i];
+        }
+        finish_columns<KIND, T, 16>(p.e, x_scales + c0, ws, b, m0 + c0, n, v);
+      }
+    }
+  }
+  if constexpr (CLUSTERED) {
+    if (!early) cluster_sync_all();  // nobody's ring is read any more
+    if (warp >= 2) {
+      const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
+      const int owner = row / slice;
+      const uint32_t mine = peer_address(inbox + static_cast<int64_t>(rank) * tokens * slice + (row - owner * slice), owner);
+      for (int c0 = 0; c0 < tokens; c0 += 16) {
+        float v[16];
+        const uint32_t at = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
+        tmem_load_16(at, v);
+        for (int c = 1; c < chains; ++c) {
+          float more[16];
+          tmem_load_16(at + c * p.tile, more);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] += more[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c0 + i < tokens) store_peer_f32(mine + static_cast<uint32_t>((c0 + i) * slice) * sizeof(float), v[i]);
+      }
+    }
+    cluster_sync_all();
+    const int r_begin = rank * slice, rows = max(0, min(kRowsW, r_begin + slice) - r_begin);
+    const int plane = tokens * slice;
+    if constexpr (KIND == GATED) {
+      const int pairs = rows / 2;
+      for (int item = threadIdx.x; item < pairs * tokens; item += kThreads) {
+        const int m = item / pairs, j = item - m * pairs;
+        const float* at = inbox + m * slice + 2 * j;
+        float gate = 0.f, up = 0.f;
+        for (int member = 0; member < members; ++member) {
+          const float2 both = *reinterpret_cast<const float2*>(at + member * plane);
+          gate += both.x;
+          up += both.y;
+        }
+        const int n = n0 + r_begin + 2 * j;
+        if (n < p.e.N) {
+          const float xs = x_scales[m];
+          const float bg = p.e.bias != nullptr ? p.e.bias[n] : 0.f, bu = p.e.bias != nullptr ? p.e.bias[n + 1] : 0.f;
+          finish_pair<T>(p.e, m0 + m, n, fmaf(gate * xs, p.e.w_scale[n], bg), fmaf(up * xs, p.e.w_scale[n + 1], bu));
+        }
+      }
+    } else {
+      for (int item = threadIdx.x; item < rows * tokens; item += kThreads) {
+        const int m = item / rows, r = item - m * rows;
+        const float* at = inbox + m * slice + r;
+        float sum = 0.f;
+        for (int member = 0; member < members; ++member) sum += at[member * plane];
+        const int n = n0 + r_begin + r;
+        if (n < p.e.N) finish_one<KIND, T>(p.e, m0 + m, n, fmaf(sum * x_scales[m], p.e.w_scale[n], p.e.bias != nullptr ? p.e.bias[n] : 0.f));
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(static_cast<uint32_t>(p.tmem_cols)) : "memory");
+  }
+}
+
+using StreamKernel = void (*)(const CUtensorMap, const CUtensorMap, const StreamParams);
+
+template <typename T, bool CLUSTERED>
+StreamKernel pick_kind(int kind) {
+  return kind == GATED ? float8_stream_kernel<GATED, T, CLUSTERED>
+         : kind == ACTIVATED ? float8_stream_kernel<ACTIVATED, T, CLUSTERED>
+                             : float8_stream_kernel<PLAIN, T, CLUSTERED>;
+}
+StreamKernel pick_kernel(int kind, bool f32, bool clustered) {
+  if (f32) return clustered ? pick_kind<float, true>(kind) : pick_kind<float, false>(kind);
+  return clustered ? pick_kind<__nv_bfloat16, true>(kind) : pick_kind<__nv_bfloat16, false>(kind);
+}
+
+constexpr size_t kMaxDynamicSmem = 200 * 1024;
+
+// An instantiation's opt-ins, once per device.
+bool prepare_kernel(StreamKernel kernel) {
+  struct Ready { StreamKernel kernel; int device; };
+  static std::mutex guard;
+  static std::vector<Ready> ready;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  std::lock_guard<std::mutex> lock(guard);
+  for (const Ready& r : ready)
+    if (r.kernel == kernel && r.device == device) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynamicSmem)) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  ready.push_back({kernel, device});
+  return true;
+}
+
+struct StreamPlan {
+  int blocks, members, tiles, tile, stages, chain_blocks, tmem_cols;
+  size_t smem;
+};
+
+// How many clusters of `members` blocks run at once with one block an SM (clusters do not straddle GPCs); 0 if it cannot be told.
+int clusters_one_per_sm(int members) {
+  const StreamKernel kernel = pick_kernel(PLAIN, false, true);
+  if (!prepare_kernel(kernel)) return 0;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(1, members * 64);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = 120 * 1024;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = 1;
+  attribute.val.clusterDim.y = members;
+  attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return clusters;
+}
+
+struct Override { int stages = 0, members = 0, target = 0, budget = 0; };
+Override g_override;  // a sweep's (b200_float8_stream_override); zeros in normal use
+
+void size_ring(StreamPlan& plan, int k_blocks, bool f32) {
+  const size_t stage = kRowsW * kBlockK + ((static_cast<size_t>(plan.tile) * kBlockK + 1023) & ~size_t(1023));
+  const int per_block = (k_blocks + plan.members - 1) / plan.members;
+  // Accumulators: one, or one per chain where outputs are 32-bit, as many as fit.
+  const int wanted = f32 ? (per_block + kChainBlocks - 1) / kChainBlocks : 1;
+  const bool alone = plan.tile > 128 || (wanted > 1 && wanted * plan.tile > 128 && plan.tile > 16);  // more than a quarter of TMEM: the SM to itself
+  const int most = alone ? 256 : 128;
+  const int accumulators = max(1, min(wanted, most / plan.tile));
+  plan.chain_blocks = (per_block + accumulators - 1) / accumulators;
+  plan.tmem_cols = 32;
+  while (plan.tmem_cols < accumulators * plan.tile) plan.tmem_cols *= 2;
+  size_t budget = alone ? 190 * 1024 : (plan.blocks * plan.members * plan.tiles <= 2 * b200_sm_count_host() ? 100 * 1024 : 66 * 1024);
+  if (g_override.budget > 0) budget = static_cast<size_t>(g_override.budget) * 1024;
+  int stages = static_cast<int>(budget / stage);
+  if (g_override.stages > 0) stages = g_override.stages;
+  stages = min(min(stages, kMaxStages), per_block);
+  plan.stages = max(stages, 2);
+  const size_t ring = plan.stages * stage;
+  const size_t inbox = plan.members > 1 ? static_cast<size_t>(plan.members) * slice_rows(plan.members) * plan.tile * sizeof(float) : 0;
+  plan.smem = (plan.tile <= kEarlyTokens ? ring + inbox : max(ring, inbox)) + 1024;
+  if (alone) plan.smem = max(plan.smem, static_cast<size_t>(118 * 1024));  // TMEM goes with shared memory: see the head of the file
+  else plan.smem = max(plan.smem, static_cast<size_t>(plan.tmem_cols) * 227 * 1024 / 512);
+}
+
+StreamPlan plan_uncached(int M, int N, int K, bool f32) {
+  StreamPlan plan;
+  plan.blocks = (N + kRowsW - 1) / kRowsW;
+  const int most = f32 ? 128 : kMaxTokens;
+  plan.tiles = (M + most - 1) / most;
+  plan.tile = (((M + plan.tiles - 1) / plan.tiles) + 15) / 16 * 16;
+  const int k_blocks = (K + kBlockK - 1) / kBlockK;
+  const int sms = b200_sm_count_host();
+  const int columns = plan.blocks * plan.tiles;
+  int target = 2 * sms;
+  if (g_override.target > 0) target = g_override.target;
+  int widest = columns * 8 < sms ? kMaxMembers : 8;
+  if (g_override.members > 0) widest = g_override.members;
+  int members = max(1, min(widest, target / columns));
+  while (members > 1 && k_blocks / members < 2) --members;  // a block keeps a few stages to stream
+  members = min(members, k_blocks);
+  plan.members = members;
+  size_ring(plan, k_blocks, f32);
+  // All clusters should run at once: one that has to wait for a place starts when the others are done.
+  if (members > 1 && g_override.members <= 0) {
+    StreamPlan narrower = plan;
+    while (narrower.members > 1) {
+      const int per_sm = max(1, min(8, static_cast<int>((227 * 1024) / (narrower.smem + 3072))));
+      const int room = clusters_one_per_sm((narrower.members + per_sm - 1) / per_sm);
+      if (room == 0 || columns <= room) break;
+      --narrower.members;
+      size_ring(narrower, k_blocks, f32);
+    }
+    if (narrower.members > 1) plan = narrower;
+  }
+  return plan;
+}
+
+// Plans are remembered: the occupancy question costs more than a launch. A plan goes by N, K and the padded tokens only.
+StreamPlan plan_stream(int M, int N, int K, bool f32) {
+  struct Entry { int m, n, k; bool f32; int device; StreamPlan plan; };
+  static std::mutex guard;
+  static std::vector<Entry> known;
+  const int rows = (M + 15) / 16 * 16;
+  int device = 0;
+  cudaGetDevice(&device);
+  std::lock_guard<std::mutex> lock(guard);
+  if (g_override.stages > 0 || g_override.members > 0 || g_override.target > 0 || g_override.budget > 0) return plan_uncached(rows, N, K, f32);
+  for (const Entry& e : known)
+    if (e.m == rows && e.n == N && e.k == K && e.f32 == f32 && e.device == device) return e.plan;
+  const StreamPlan plan = plan_uncached(rows, N, K, f32);
+  if (known.size() >= 4096) known.clear();
+  known.push_back({rows, N, K, f32, device, plan});
+  return plan;
+}
+
+}  // namespace
+
+int launch_stream(const Product& product, cudaStream_t stream) {
+  const Epilogue& e = product.e;
+  const bool f32 = product.out_f32 != 0;
+  const StreamPlan plan = plan_stream(e.M, e.N, product.K, f32);
+  B200_REQUIRE(plan.smem <= kMaxDynamicSmem, "float8 product: the plan wants %zu bytes of shared memory", plan.smem);
+  StreamParams p;
+  p.e = e;
+  p.err = product.err;
+  p.K = product.K;
+  p.stages = plan.stages;
+  p.tile = plan.tile;
+  p.chain_blocks = plan.chain_blocks;
+  p.tmem_cols = plan.tmem_cols;
+  p.w_constant = product.w_constant;
+  CUtensorMap w_map, x_map;
+  if (make_map(&w_map, product.w, e.N, product.K, product.w_stride, kRowsW) != 0) return -1;
+  if (make_map(&x_map, product.x, e.M, product.K, product.x_stride, plan.tile) != 0) return -1;
+  const StreamKernel kernel = pick_kernel(product.kind, f32, plan.members > 1);
+  if (!prepare_kernel(kernel)) return b200_fail("float8 product: the kernel's attributes could not be set");
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(plan.blocks, plan.members, plan.tiles);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = plan.smem;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  int count = 0;
+  if (plan.members > 1) {
+    attributes[count].id = cudaLaunchAttributeClusterDimension;
+    attributes[count].val.clusterDim.x = 1;
+    attributes[count].val.clusterDim.y = plan.members;
+    attributes[count].val.clusterDim.z = 1;
+    ++count;
+  }
+  if (b200_overlap_enabled()) {
+    attributes[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[count].val.programmaticStreamSerializationAllowed = 1;
+    ++count;
+  }
+  config.attrs = attributes;
+  config.numAttrs = count;
+  const cudaError_t status = cudaLaunchKernelEx(&config, kernel, w_map, x_map, p);
+  if (status != cudaSuccess) {
+    cudaGetLastError();
+    return b200_fail("float8 product: %s", cudaGetErrorString(status));
+  }
+  return 0;
+}
+
+}  // namespace float8
+
+// For parameter sweeps only: force the ring depth, the cluster width, the blocks aimed at or the ring's budget in KB (0: the planner's own).
+B200_API void b200_float8_stream_override(int stages, int members, int target, int budget) {
+  float8::g_override = {stages, members, target, budget};
+}

@@ -50,6 +50,10 @@ def stream_handle() -> c_void_p:
 _SIGNATURES: dict[str, list] = {
     "b200_embedding_gather": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p],
     "b200_rmsnorm": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_void_p],
+    "b200_float8_quantize": [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p],
+    "b200_float8_rmsnorm": [c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p],
+    "b200_float8_linear": [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64]
+    + [c_int] * 5 + [c_void_p, c_void_p],
     "b200_silu_mul": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "b200_gelu_mul": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "b200_rope_kv_write": [c_void_p] * 7 + [c_int, c_int] + [c_void_p] * 3 + [c_int] * 8 + [c_void_p, c_void_p],
