@@ -38,7 +38,7 @@ struct Epilogue {
   int64_t residual_stride;
   int M, N;
   int activation;
-  int pairs;  // bfloat16 rows can be written two numbers at a time: N and the stride even, the base on 4 bytes
+  int pairs;  // rows can be written two numbers at a time: N and the stride even, the base on two numbers' boundary
 };
 
 __device__ __forceinline__ float activate(float v, int activation) {
@@ -47,58 +47,85 @@ __device__ __forceinline__ float activate(float v, int activation) {
   const float r = v < 0.f ? 0.f : v;  // NaN stays
   return r * r;
 }
-__device__ __forceinline__ float gate_times_up(float gate, float up, int activation) {
-  return activation == ACT_GELU ? gated_unit<true>(gate, up) : gated_unit<false>(gate, up);
-}
-
-// One output of a product that is not gated, from the sum with its scales and bias.
-template <int KIND, typename T>
-__device__ __forceinline__ void finish_one(const Epilogue& e, int m, int n, float v) {
-  if constexpr (KIND == ACTIVATED) v = activate(v, e.activation);
-  if (e.residual != nullptr) v += e.residual[m * e.residual_stride + n];
-  static_cast<T*>(e.out)[m * e.out_stride + n] = from_f32<T>(v);
-}
-template <typename T>
-__device__ __forceinline__ void finish_pair(const Epilogue& e, int m, int n, float gate, float up) {  // n: the gate's row of W
-  static_cast<T*>(e.out)[m * e.out_stride + (n >> 1)] = from_f32<T>(gate_times_up(gate, up, e.activation));
+// `COUNT` sums with their scales and bias through the activation; the choice is the call's, so it is made once.
+template <int COUNT>
+__device__ __forceinline__ void activate_all(float (&v)[COUNT], int activation) {
+  if (activation == ACT_SQUARED_RELU) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] = activate(v[i], ACT_SQUARED_RELU);
+  } else if (activation == ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] = activate(v[i], ACT_SILU);
+  } else {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] = activate(v[i], ACT_GELU);
+  }
 }
 
 // COUNT tokens from m0 on, one per entry of `v` (sums without scales), for the row of W that this lane holds (n; 32 neighbouring rows a
-// warp, n0 even for lane 0). `xs` are the tokens' scales, ws and b the row's own. Rows are features, so a warp's store covers 32 neighbours of
-// one output row. bfloat16 neighbours trade one of two tokens with the lane beside them, and each then stores 4 bytes instead of two times 2;
-// in gated products the same trade brings a gate and its up value together. The whole warp calls this.
+// warp, even for lane 0). `xs` are the tokens' scales (16-byte aligned), ws and b the row's own. Rows are features, so a warp's store covers 32
+// neighbours of one output row. bfloat16 neighbours trade one of two tokens with the lane beside them, and each then stores 4 bytes instead of two
+// times 2; in gated products the same trade brings a gate and its up value together. All of it is straight-line code, the residual asked for
+// first: with a branch per pair of tokens, and each residual number loaded where it is added, a tile of 128 x 256 took 8 us instead of 2.
+// The whole warp calls this.
 template <int KIND, typename T, int COUNT>
-__device__ __forceinline__ void finish_columns(const Epilogue& e, const float* xs, float ws, float b, int m0, int n, const float (&v)[COUNT]) {
-  const bool odd = threadIdx.x & 1;
+__device__ __forceinline__ void finish_columns(const Epilogue& e, const float* xs, float ws, float b, int m0, int n, float (&v)[COUNT]) {
+  const bool odd = threadIdx.x & 1, live = n < e.N;
+  const int count = min(COUNT, e.M - m0);  // tokens there are
+  float r[COUNT];
+  const bool add = KIND != GATED && e.residual != nullptr;
+  if (add) {
+    const float* from = e.residual + m0 * e.residual_stride + n;
 #pragma unroll
-  for (int i = 0; i < COUNT; i += 2) {
-    if (m0 + i >= e.M) break;
-    float first = fmaf(v[i] * xs[i], ws, b), second = fmaf(v[i + 1] * xs[i + 1], ws, b);
-    if constexpr (KIND == GATED) {
-      const float other = __shfl_xor_sync(0xffffffffu, odd ? first : second, 1);
-      const int m = m0 + i + odd;
-      if (m < e.M && n < e.N) finish_pair<T>(e, m, n, odd ? other : first, odd ? second : other);
-    } else {
-      if (sizeof(T) == 2 && e.pairs) {
-        if constexpr (KIND == ACTIVATED) {
-          first = activate(first, e.activation);
-          second = activate(second, e.activation);
-        }
-        if (e.residual != nullptr && n < e.N) {
-          const float* r = e.residual + (m0 + i) * e.residual_stride + n;
-          first += r[0];
-          if (m0 + i + 1 < e.M) second += r[e.residual_stride];
-        }
-        const float other = __shfl_xor_sync(0xffffffffu, odd ? first : second, 1);
-        const int m = m0 + i + odd;
-        if (m < e.M && n < e.N)
-          *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(e.out) + m * e.out_stride + (n & ~1)) =
-              odd ? __floats2bfloat162_rn(other, second) : __floats2bfloat162_rn(first, other);
-      } else if (n < e.N) {
-        finish_one<KIND, T>(e, m0 + i, n, first);
-        if (m0 + i + 1 < e.M) finish_one<KIND, T>(e, m0 + i + 1, n, second);
-      }
+    for (int i = 0; i < COUNT; ++i) r[i] = live && i < count ? from[i * e.residual_stride] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < COUNT; i += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(xs + i);
+    v[i] = fmaf(v[i] * s.x, ws, b);
+    v[i + 1] = fmaf(v[i + 1] * s.y, ws, b);
+    v[i + 2] = fmaf(v[i + 2] * s.z, ws, b);
+    v[i + 3] = fmaf(v[i + 3] * s.w, ws, b);
+  }
+  if constexpr (KIND == ACTIVATED) activate_all<COUNT>(v, e.activation);
+  if (add) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] += r[i];
+  }
+  T* to = static_cast<T*>(e.out) + m0 * e.out_stride;
+  if constexpr (KIND == GATED) {
+    float y[COUNT / 2];  // this lane's gate-and-up pairs: tokens 2 i + odd
+#pragma unroll
+    for (int i = 0; i < COUNT; i += 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
+      const float gate = odd ? other : v[i], up = odd ? v[i + 1] : other;
+      v[i] = gate;
+      v[i + 1] = up;
     }
+    if (e.activation == ACT_GELU) {
+#pragma unroll
+      for (int i = 0; i < COUNT / 2; ++i) y[i] = gated_unit<true>(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < COUNT / 2; ++i) y[i] = gated_unit<false>(v[2 * i], v[2 * i + 1]);
+    }
+    to += odd * e.out_stride + (n >> 1);
+#pragma unroll
+    for (int i = 0; i < COUNT / 2; ++i)
+      if (live && 2 * i + odd < count) to[2 * i * e.out_stride] = from_f32<T>(y[i]);
+  } else if (sizeof(T) == 2 && e.pairs) {
+    __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(to) + odd * e.out_stride + (n & ~1);
+#pragma unroll
+    for (int i = 0; i < COUNT; i += 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
+      if (live && i + odd < count)
+        *reinterpret_cast<__nv_bfloat162*>(at + i * e.out_stride) = odd ? __floats2bfloat162_rn(other, v[i + 1]) : __floats2bfloat162_rn(v[i], other);
+    }
+  } else {
+    to += n;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      if (live && i < count) to[i * e.out_stride] = from_f32<T>(v[i]);
   }
 }
 
@@ -155,17 +182,33 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(chosen));
   return chosen != 0;
 }
-__device__ __forceinline__ void tmem_load_16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
+// 16 columns of this warp's 32 TMEM lanes, a lane per thread: asked for, and there once tmem_wait has returned.
+__device__ __forceinline__ void tmem_ask_16(uint32_t taddr, float (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
       : "r"(taddr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait(float (&v)[16]) {  // the numbers go through it, so that none is used before
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
+// The same 16 columns of `chains` accumulators, `apart` columns from one to the next, added in order.
+__device__ __forceinline__ void tmem_sums_16(uint32_t taddr, int chains, int apart, float (&v)[16]) {
+  tmem_ask_16(taddr, v);
+  tmem_wait(v);
+  for (int c = 1; c < chains; ++c) {
+    float more[16];
+    tmem_ask_16(taddr + c * apart, more);
+    tmem_wait(more);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 16; ++i) v[i] += more[i];
+  }
 }
 
 // --- host ------------------------------------------------------------------------------------------
@@ -188,6 +231,6 @@ struct Product {
 // csrc/kernels/gemm_float8_stream.cu: weights streamed past few tokens, K split inside clusters.
 int launch_stream(const Product& p, cudaStream_t stream);
 // csrc/kernels/gemm_float8_tiles.cu: pairs of SMs on tiles of 256 rows of W by up to 256 tokens.
-int launch_tiles(const Product& p, cudaStream_t stream);
+int launch_tiles(const Product& p, int tile, cudaStream_t stream);
 
 }  // namespace float8

@@ -3,6 +3,7 @@
 
 namespace float8 {
 
+int g_tile = 0;
 namespace {
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -54,6 +55,8 @@ B200_API int b200_float8_linear(const void* x, int64_t x_stride, const float* x_
   p.x = x, p.w = w, p.x_stride = x_stride, p.w_stride = w_stride, p.K = K, p.kind = kind, p.out_f32 = out_dtype == DTYPE_F32, p.w_constant = w_constant, p.err = err;
   p.e.out = out, p.e.x_scale = x_scale, p.e.w_scale = w_scale, p.e.bias = bias, p.e.residual = residual;
   p.e.out_stride = out_stride, p.e.residual_stride = residual_stride, p.e.M = M, p.e.N = N, p.e.activation = activation;
-  p.e.pairs = N % 2 == 0 && out_stride % 2 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
+  p.e.pairs = N % 2 == 0 && out_stride % 2 == 0 && reinterpret_cast<uintptr_t>(out) % (out_dtype == DTYPE_F32 ? 8 : 4) == 0;
+  if (float8::g_tile > 0) return launch_tiles(p, float8::g_tile, stream);
   return launch_stream(p, stream);
 }
+B200_API void b200_float8_tile_override(int tile) { float8::g_tile = tile; }

@@ -40,8 +40,8 @@ struct StreamParams {
   int w_constant;
 };
 
-// Rows of a block that one member of a cluster finishes; gate and up stay together.
-__host__ __device__ constexpr int slice_rows(int members) { return (((kRowsW + members - 1) / members) + 1) & ~1; }
+// Rows of a block that one member of a cluster finishes: whole 32-byte pieces of 32-bit output rows (the last members may have none).
+__host__ __device__ constexpr int slice_rows(int members) { return ((kRowsW + members - 1) / members + 7) & ~7; }
 
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
   asm volatile(
@@ -54,6 +54,65 @@ __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a_desc, uint64_t 
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// What one member finishes: `rows` rows of W from n0 on, the members' partial sums ([members][tokens][slice]) added in member order. An item is two
+// neighbouring rows of one token; a thread takes kItems of them at a time and asks for everything from memory before it adds.
+template <int KIND, typename T>
+__device__ __forceinline__ void finish_slice(const Epilogue& e, const float* inbox, const float* x_scales, int m0, int tokens, int n0, int rows, int slice, int members) {
+  constexpr int kItems = 4;
+  const int pairs = min(rows, e.N - n0 + 1) / 2;  // with rows of W left
+  const int total = pairs * tokens, plane = tokens * slice;
+  for (int base = threadIdx.x; base < total; base += kThreads * kItems) {
+    int m[kItems], j[kItems];
+    float2 sum[kItems], ws[kItems], b[kItems], r[kItems];
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const int item = min(base + u * kThreads, total - 1);
+      m[u] = item / pairs;
+      j[u] = 2 * (item - m[u] * pairs);
+      const int n = n0 + j[u];
+      const bool second = n + 1 < e.N;
+      ws[u] = make_float2(e.w_scale[n], second ? e.w_scale[n + 1] : 0.f);
+      b[u] = e.bias != nullptr ? make_float2(e.bias[n], second ? e.bias[n + 1] : 0.f) : make_float2(0.f, 0.f);
+      r[u] = make_float2(0.f, 0.f);
+      if (KIND != GATED && e.residual != nullptr && base + u * kThreads < total) {
+        const float* from = e.residual + (m0 + m[u]) * e.residual_stride + n;
+        r[u] = make_float2(from[0], second ? from[1] : 0.f);
+      }
+      sum[u] = make_float2(0.f, 0.f);
+    }
+    for (int member = 0; member < members; ++member) {
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) {
+        const float2 part = *reinterpret_cast<const float2*>(inbox + member * plane + m[u] * slice + j[u]);
+        sum[u].x += part.x;
+        sum[u].y += part.y;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      if (base + u * kThreads >= total) break;
+      const float xs = x_scales[m[u]];
+      const int n = n0 + j[u];
+      float v[2] = {fmaf(sum[u].x * xs, ws[u].x, b[u].x), fmaf(sum[u].y * xs, ws[u].y, b[u].y)};
+      T* to = static_cast<T*>(e.out) + (m0 + m[u]) * e.out_stride;
+      if constexpr (KIND == GATED) {
+        to[n >> 1] = from_f32<T>(e.activation == ACT_GELU ? gated_unit<true>(v[0], v[1]) : gated_unit<false>(v[0], v[1]));
+      } else {
+        if constexpr (KIND == ACTIVATED) activate_all<2>(v, e.activation);
+        v[0] += r[u].x;
+        v[1] += r[u].y;
+        if (e.pairs) {
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to + n) = make_float2(v[0], v[1]);
+          else *reinterpret_cast<__nv_bfloat162*>(to + n) = __floats2bfloat162_rn(v[0], v[1]);
+        } else {
+          to[n] = from_f32<T>(v[0]);
+          if (n + 1 < e.N) to[n + 1] = from_f32<T>(v[1]);
+        }
+      }
+    }
+  }
 }
 
 // A form carries no code that it does not take: a block runs its epilogue once, from a cold instruction cache (measured in gemm_tcgen05.cu).
@@ -69,7 +128,7 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   __shared__ __align__(8) uint64_t empty_bar[kMaxStages];
   __shared__ __align__(8) uint64_t accum_bar;
   __shared__ uint32_t tmem_base_shared;
-  __shared__ float x_scales[kMaxTokens];
+  __shared__ __align__(16) float x_scales[kMaxTokens];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int stages = p.stages;
@@ -180,14 +239,7 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
       for (int c0 = 0; have && c0 < tokens; c0 += 16) {
         float v[16];
-        const uint32_t at = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
-        tmem_load_16(at, v);
-        for (int c = 1; c < chains; ++c) {
-          float more[16];
-          tmem_load_16(at + c * p.tile, more);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] += more[i];
-        }
+        tmem_sums_16(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, chains, p.tile, v);
         finish_columns<KIND, T, 16>(p.e, x_scales + c0, ws, b, m0 + c0, n, v);
       }
     }
@@ -200,50 +252,14 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       const uint32_t mine = peer_address(inbox + static_cast<int64_t>(rank) * tokens * slice + (row - owner * slice), owner);
       for (int c0 = 0; c0 < tokens; c0 += 16) {
         float v[16];
-        const uint32_t at = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
-        tmem_load_16(at, v);
-        for (int c = 1; c < chains; ++c) {
-          float more[16];
-          tmem_load_16(at + c * p.tile, more);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] += more[i];
-        }
+        tmem_sums_16(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, chains, p.tile, v);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (c0 + i < tokens) store_peer_f32(mine + static_cast<uint32_t>((c0 + i) * slice) * sizeof(float), v[i]);
       }
     }
     cluster_sync_all();
-    const int r_begin = rank * slice, rows = max(0, min(kRowsW, r_begin + slice) - r_begin);
-    const int plane = tokens * slice;
-    if constexpr (KIND == GATED) {
-      const int pairs = rows / 2;
-      for (int item = threadIdx.x; item < pairs * tokens; item += kThreads) {
-        const int m = item / pairs, j = item - m * pairs;
-        const float* at = inbox + m * slice + 2 * j;
-        float gate = 0.f, up = 0.f;
-        for (int member = 0; member < members; ++member) {
-          const float2 both = *reinterpret_cast<const float2*>(at + member * plane);
-          gate += both.x;
-          up += both.y;
-        }
-        const int n = n0 + r_begin + 2 * j;
-        if (n < p.e.N) {
-          const float xs = x_scales[m];
-          const float bg = p.e.bias != nullptr ? p.e.bias[n] : 0.f, bu = p.e.bias != nullptr ? p.e.bias[n + 1] : 0.f;
-          finish_pair<T>(p.e, m0 + m, n, fmaf(gate * xs, p.e.w_scale[n], bg), fmaf(up * xs, p.e.w_scale[n + 1], bu));
-        }
-      }
-    } else {
-      for (int item = threadIdx.x; item < rows * tokens; item += kThreads) {
-        const int m = item / rows, r = item - m * rows;
-        const float* at = inbox + m * slice + r;
-        float sum = 0.f;
-        for (int member = 0; member < members; ++member) sum += at[member * plane];
-        const int n = n0 + r_begin + r;
-        if (n < p.e.N) finish_one<KIND, T>(p.e, m0 + m, n, fmaf(sum * x_scales[m], p.e.w_scale[n], p.e.bias != nullptr ? p.e.bias[n] : 0.f));
-      }
-    }
+    finish_slice<KIND, T>(p.e, inbox, x_scales, m0, tokens, n0 + rank * slice, max(0, min(kRowsW - rank * slice, slice)), slice, members);
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
