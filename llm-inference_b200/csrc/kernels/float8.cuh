@@ -4,14 +4,15 @@
 // row; the number at (row, k) is q * scale. A product of two such matrices has both scales in front of the sum:
 //   y[m][n] = (sum_k x[m][k] w[n][k]) * xs[m] * ws[n].
 // A product of two e4m3 numbers has 8 bits, so every product is exact; sums are 32-bit. `tcgen05.mma` drops the bits below the last when it
-// adds (toward zero), which over a chain of n additions makes a sum smaller by about n 2^-25 of itself: 1e-5 after the 592 additions of
-// K = 18,944. Where outputs are 32-bit the chains are therefore cut (kChainBlocks) and the pieces added in registers with ordinary
-// rounding; a bfloat16 output's own rounding (2^-9) is a hundred times what an uncut chain loses.
+// adds (toward zero). Measured, a chain of n additions (32 k each) makes a sum of numbers of both signs smaller by 1.6e-9 n of itself, of one sign by
+// 1.5e-8 n: 5e-7 and 4.3e-6 for n = 296. Where outputs are 32-bit the chains are therefore cut after 64 additions (kChainBlocks) and
+// the pieces added in registers with ordinary rounding; a bfloat16 output's own rounding (2^-9) is hundreds of times what an uncut chain loses.
 #pragma once
 
 #include <cuda.h>
 
 #include "common.cuh"
+#include "packs.cuh"
 
 namespace float8 {
 
@@ -20,7 +21,7 @@ constexpr float kSmallestScale = 1.17549435e-38f;  // 2^-126: a row of zeros has
 constexpr int kRowsW = 128;                   // rows of W a block holds: TMEM lanes
 constexpr int kBlockK = 128;                  // k per stage: 128 bytes, one swizzle row
 constexpr int kMmaK = 32;
-constexpr int kChainBlocks = 4;               // 32-bit outputs: k-blocks a chain runs over (16 additions: 5e-7 of a sum at most)
+constexpr int kChainBlocks = 16;              // 32-bit outputs: k-blocks a chain runs over (64 additions)
 constexpr long long kWaitCycles = 4000000000LL;  // about two seconds
 constexpr int ERRBIT_TIMEOUT = 8;
 
@@ -38,7 +39,7 @@ struct Epilogue {
   int64_t residual_stride;
   int M, N;
   int activation;
-  int pairs;  // rows can be written two numbers at a time: N and the stride even, the base on two numbers' boundary
+  int vector;  // four neighbouring outputs of a row can be written (and residuals read) at once: strides and bases allow it
 };
 
 __device__ __forceinline__ float activate(float v, int activation) {
@@ -47,87 +48,151 @@ __device__ __forceinline__ float activate(float v, int activation) {
   const float r = v < 0.f ? 0.f : v;  // NaN stays
   return r * r;
 }
-// `COUNT` sums with their scales and bias through the activation; the choice is the call's, so it is made once.
-template <int COUNT>
-__device__ __forceinline__ void activate_all(float (&v)[COUNT], int activation) {
-  if (activation == ACT_SQUARED_RELU) {
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) v[i] = activate(v[i], ACT_SQUARED_RELU);
-  } else if (activation == ACT_SILU) {
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) v[i] = activate(v[i], ACT_SILU);
+
+// Four neighbouring outputs (n a multiple of four, rows of W beyond the last left out): the residual's, and from four sums with their scales and bias.
+__device__ __forceinline__ float4 residual_quad(const Epilogue& e, int m, int n) {
+  const float* from = e.residual + m * e.residual_stride + n;
+  if (e.vector && n + 3 < e.N) return *reinterpret_cast<const float4*>(from);
+  return make_float4(n < e.N ? from[0] : 0.f, n + 1 < e.N ? from[1] : 0.f, n + 2 < e.N ? from[2] : 0.f, n + 3 < e.N ? from[3] : 0.f);
+}
+__device__ __forceinline__ float4 activate_quad(float4 v, int activation) {
+  return make_float4(activate(v.x, activation), activate(v.y, activation), activate(v.z, activation), activate(v.w, activation));
+}
+__device__ __forceinline__ float2 gated_pair(float4 v, int activation) {  // gate, up, gate, up
+  return activation == ACT_GELU ? make_float2(gated_unit<true>(v.x, v.y), gated_unit<true>(v.z, v.w))
+                                : make_float2(gated_unit<false>(v.x, v.y), gated_unit<false>(v.z, v.w));
+}
+// Four finished numbers (gated: still gates and up values) to their place: all of them on an aligned place, or those that belong to rows of W.
+template <int KIND, typename T>
+__device__ __forceinline__ void store_whole(T* to, float4 v, int activation) {
+  if constexpr (KIND == GATED) {
+    const float2 y = gated_pair(v, activation);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = y;
+    else *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(y.x, y.y);
   } else {
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) v[i] = activate(v[i], ACT_GELU);
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(to) = v;
+    } else {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+      *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+  }
+}
+template <int KIND, typename T>
+__device__ __noinline__ void store_some(T* to, int n, int N, float4 v, int activation) {
+  if constexpr (KIND == GATED) {
+    const float2 y = gated_pair(v, activation);
+    if (n < N) to[0] = from_f32<T>(y.x);
+    if (n + 2 < N) to[1] = from_f32<T>(y.y);
+  } else {
+    if (n < N) to[0] = from_f32<T>(v.x);
+    if (n + 1 < N) to[1] = from_f32<T>(v.y);
+    if (n + 2 < N) to[2] = from_f32<T>(v.z);
+    if (n + 3 < N) to[3] = from_f32<T>(v.w);
   }
 }
 
-// COUNT tokens from m0 on, one per entry of `v` (sums without scales), for the row of W that this lane holds (n; 32 neighbouring rows a
-// warp, even for lane 0). `xs` are the tokens' scales (16-byte aligned), ws and b the row's own. Rows are features, so a warp's store covers 32
-// neighbours of one output row. bfloat16 neighbours trade one of two tokens with the lane beside them, and each then stores 4 bytes instead of two
-// times 2; in gated products the same trade brings a gate and its up value together. All of it is straight-line code, the residual asked for
-// first: with a branch per pair of tokens, and each residual number loaded where it is added, a tile of 128 x 256 took 8 us instead of 2.
-// The whole warp calls this.
-template <int KIND, typename T, int COUNT>
-__device__ __forceinline__ void finish_columns(const Epilogue& e, const float* xs, float ws, float b, int m0, int n, float (&v)[COUNT]) {
-  const bool odd = threadIdx.x & 1, live = n < e.N;
-  const int count = min(COUNT, e.M - m0);  // tokens there are
-  float r[COUNT];
-  const bool add = KIND != GATED && e.residual != nullptr;
-  if (add) {
-    const float* from = e.residual + m0 * e.residual_stride + n;
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) r[i] = live && i < count ? from[i * e.residual_stride] : 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < COUNT; i += 4) {
-    const float4 s = *reinterpret_cast<const float4*>(xs + i);
-    v[i] = fmaf(v[i] * s.x, ws, b);
-    v[i + 1] = fmaf(v[i + 1] * s.y, ws, b);
-    v[i + 2] = fmaf(v[i + 2] * s.z, ws, b);
-    v[i + 3] = fmaf(v[i + 3] * s.w, ws, b);
-  }
-  if constexpr (KIND == ACTIVATED) activate_all<COUNT>(v, e.activation);
-  if (add) {
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) v[i] += r[i];
-  }
-  T* to = static_cast<T*>(e.out) + m0 * e.out_stride;
-  if constexpr (KIND == GATED) {
-    float y[COUNT / 2];  // this lane's gate-and-up pairs: tokens 2 i + odd
-#pragma unroll
-    for (int i = 0; i < COUNT; i += 2) {
-      const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
-      const float gate = odd ? other : v[i], up = odd ? v[i + 1] : other;
-      v[i] = gate;
-      v[i + 1] = up;
-    }
-    if (e.activation == ACT_GELU) {
-#pragma unroll
-      for (int i = 0; i < COUNT / 2; ++i) y[i] = gated_unit<true>(v[2 * i], v[2 * i + 1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < COUNT / 2; ++i) y[i] = gated_unit<false>(v[2 * i], v[2 * i + 1]);
-    }
-    to += odd * e.out_stride + (n >> 1);
-#pragma unroll
-    for (int i = 0; i < COUNT / 2; ++i)
-      if (live && 2 * i + odd < count) to[2 * i * e.out_stride] = from_f32<T>(y[i]);
-  } else if (sizeof(T) == 2 && e.pairs) {
-    __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(to) + odd * e.out_stride + (n & ~1);
-#pragma unroll
-    for (int i = 0; i < COUNT; i += 2) {
-      const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
-      if (live && i + odd < count)
-        *reinterpret_cast<__nv_bfloat162*>(at + i * e.out_stride) = odd ? __floats2bfloat162_rn(other, v[i + 1]) : __floats2bfloat162_rn(v[i], other);
-    }
-  } else {
-    to += n;
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i)
-      if (live && i < count) to[i * e.out_stride] = from_f32<T>(v[i]);
-  }
+// Two 32-bit numbers at once.
+__device__ __forceinline__ float2 mul_2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}\n" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
 }
+__device__ __forceinline__ float2 fma_2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+// A warp's way out of TMEM: 32 neighbouring rows of W, one a lane (n0: lane 0's, a multiple of 32), for tokens m0, m0 + 1, ..., eight at a time. The
+// numbers pass through `stage`, 1 KB of shared memory of the warp's own, so that a lane goes on with four neighbouring rows of one token: a
+// quarter of the stores, addresses and conditions, and gates beside their up values. (Neighbours that trade numbers by shuffles took 13
+// instructions an output and 3.6 us for the 128 x 256 sums of an SM, eight warps; this takes under five.) The whole warp calls this.
+constexpr int kStageFloats = 8 * 32;
+template <int KIND, typename T>
+class WayOut {
+ public:
+  __device__ __forceinline__ WayOut(const Epilogue& e, int m0, int n0, float* stage) : e_(e), stage_(stage) {
+    const int lane = threadIdx.x & 31;
+    ws_ = b_ = 0.f;
+    if (n0 + lane < e.N) {
+      ws_ = e.w_scale[n0 + lane];
+      if (e.bias != nullptr) b_ = e.bias[n0 + lane];
+    }
+    m_ = m0;
+    n_ = n0 + (lane & 7) * 4;
+    whole_ = e.vector && n0 + 31 < e.N;
+    const int m = m0 + (lane >> 3);  // this lane's tokens: m, m + 4 of each eight
+    to_ = static_cast<T*>(e.out) + m * e.out_stride + (KIND == GATED ? n_ >> 1 : n_);
+    from_ = e.residual != nullptr ? e.residual + m * e.residual_stride + n_ : nullptr;
+  }
+
+  // The next eight tokens; `v`: sums without scales, `xs`: the tokens' scales (16-byte aligned).
+  __device__ __forceinline__ void take(const float* xs, const float (&v)[8]) {
+    const int lane = threadIdx.x & 31;
+    const int left = e_.M - m_;
+    const bool whole = whole_ && left >= 8;
+    float4 r[2];
+    if (KIND != GATED && e_.residual != nullptr) {
+      if (whole) {
+        r[0] = *reinterpret_cast<const float4*>(from_);
+        r[1] = *reinterpret_cast<const float4*>(from_ + 4 * e_.residual_stride);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) r[q] = q * 4 + (lane >> 3) < left ? residual_quad(e_, m_ + q * 4 + (lane >> 3), n_) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      from_ += 8 * e_.residual_stride;
+    }
+    const float2 ws = make_float2(ws_, ws_), b = make_float2(b_, b_);
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(xs + i);
+      const float2 lo = fma_2(mul_2(make_float2(v[i], v[i + 1]), make_float2(s.x, s.y)), ws, b);
+      const float2 hi = fma_2(mul_2(make_float2(v[i + 2], v[i + 3]), make_float2(s.z, s.w)), ws, b);
+      stage_[i * 32 + lane] = lo.x;
+      stage_[(i + 1) * 32 + lane] = lo.y;
+      stage_[(i + 2) * 32 + lane] = hi.x;
+      stage_[(i + 3) * 32 + lane] = hi.y;
+    }
+    __syncwarp();
+    float4 mine[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) mine[q] = *reinterpret_cast<const float4*>(stage_ + (q * 4 + (lane >> 3)) * 32 + (lane & 7) * 4);
+    if (KIND != GATED && KIND != ACTIVATED && e_.residual != nullptr) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) mine[q] = add_each(mine[q], r[q]);
+    }
+    if constexpr (KIND == ACTIVATED) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        mine[q] = activate_quad(mine[q], e_.activation);
+        if (e_.residual != nullptr) mine[q] = add_each(mine[q], r[q]);
+      }
+    }
+    if (whole) {
+      store_whole<KIND, T>(to_, mine[0], e_.activation);
+      store_whole<KIND, T>(to_ + 4 * e_.out_stride, mine[1], e_.activation);
+    } else {
+#pragma unroll 1
+      for (int q = 0; q < 2; ++q)
+        if (q * 4 + (lane >> 3) < left) store_some<KIND, T>(to_ + q * 4 * e_.out_stride, n_, e_.N, q == 0 ? mine[0] : mine[1], e_.activation);
+    }
+    to_ += 8 * e_.out_stride;
+    m_ += 8;
+    __syncwarp();
+  }
+
+ private:
+  const Epilogue& e_;
+  float* stage_;
+  float ws_, b_;
+  int m_, n_;
+  bool whole_;
+  T* to_;
+  const float* from_;
+};
 
 // --- shared memory, TMA, tcgen05 -------------------------------------------------------------------
 
@@ -182,32 +247,35 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(chosen));
   return chosen != 0;
 }
-// 16 columns of this warp's 32 TMEM lanes, a lane per thread: asked for, and there once tmem_wait has returned.
-__device__ __forceinline__ void tmem_ask_16(uint32_t taddr, float (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
-        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-      : "r"(taddr)
-      : "memory");
+// Eight columns of this warp's 32 TMEM lanes, a lane per thread: asked for, and there once tmem_wait has returned.
+__device__ __forceinline__ void tmem_ask(uint32_t taddr, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(taddr)
+               : "memory");
 }
-__device__ __forceinline__ void tmem_wait(float (&v)[16]) {  // the numbers go through it, so that none is used before
+__device__ __forceinline__ void tmem_wait(float (&v)[8]) {  // the numbers go through it, so that none is used before
   asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])
                :
                : "memory");
 }
-// The same 16 columns of `chains` accumulators, `apart` columns from one to the next, added in order.
-__device__ __forceinline__ void tmem_sums_16(uint32_t taddr, int chains, int apart, float (&v)[16]) {
-  tmem_ask_16(taddr, v);
+__device__ __forceinline__ void tmem_store(uint32_t taddr, const float (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The same eight columns of `chains` accumulators, `apart` columns from one to the next, added in order.
+__device__ __forceinline__ void tmem_sums(uint32_t taddr, int chains, int apart, float (&v)[8]) {
+  tmem_ask(taddr, v);
   tmem_wait(v);
   for (int c = 1; c < chains; ++c) {
-    float more[16];
-    tmem_ask_16(taddr + c * apart, more);
+    float more[8];
+    tmem_ask(taddr + c * apart, more);
     tmem_wait(more);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] += more[i];
+    for (int i = 0; i < 8; ++i) v[i] += more[i];
   }
 }
 

@@ -55,7 +55,9 @@ B200_API int b200_float8_linear(const void* x, int64_t x_stride, const float* x_
   p.x = x, p.w = w, p.x_stride = x_stride, p.w_stride = w_stride, p.K = K, p.kind = kind, p.out_f32 = out_dtype == DTYPE_F32, p.w_constant = w_constant, p.err = err;
   p.e.out = out, p.e.x_scale = x_scale, p.e.w_scale = w_scale, p.e.bias = bias, p.e.residual = residual;
   p.e.out_stride = out_stride, p.e.residual_stride = residual_stride, p.e.M = M, p.e.N = N, p.e.activation = activation;
-  p.e.pairs = N % 2 == 0 && out_stride % 2 == 0 && reinterpret_cast<uintptr_t>(out) % (out_dtype == DTYPE_F32 ? 8 : 4) == 0;
+  const int size = out_dtype == DTYPE_F32 ? 4 : 2, at_once = kind == GATED ? 2 : 4;  // outputs from four rows of W
+  p.e.vector = out_stride % at_once == 0 && reinterpret_cast<uintptr_t>(out) % (at_once * size) == 0 &&
+               (residual == nullptr || (residual_stride % 4 == 0 && reinterpret_cast<uintptr_t>(residual) % 16 == 0));
   if (float8::g_tile > 0) return launch_tiles(p, float8::g_tile, stream);
   return launch_stream(p, stream);
 }

@@ -56,61 +56,47 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
-// What one member finishes: `rows` rows of W from n0 on, the members' partial sums ([members][tokens][slice]) added in member order. An item is two
+// What one member finishes: `rows` rows of W from n0 on, the members' partial sums ([members][tokens][slice]) added in member order. An item is four
 // neighbouring rows of one token; a thread takes kItems of them at a time and asks for everything from memory before it adds.
 template <int KIND, typename T>
 __device__ __forceinline__ void finish_slice(const Epilogue& e, const float* inbox, const float* x_scales, int m0, int tokens, int n0, int rows, int slice, int members) {
-  constexpr int kItems = 4;
-  const int pairs = min(rows, e.N - n0 + 1) / 2;  // with rows of W left
-  const int total = pairs * tokens, plane = tokens * slice;
+  constexpr int kItems = 2;
+  const int quads = (min(rows, e.N - n0) + 3) / 4;  // with rows of W left
+  const int total = quads * tokens, plane = tokens * slice;
   for (int base = threadIdx.x; base < total; base += kThreads * kItems) {
     int m[kItems], j[kItems];
-    float2 sum[kItems], ws[kItems], b[kItems], r[kItems];
+    float4 sum[kItems], ws[kItems], b[kItems], r[kItems];
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
       const int item = min(base + u * kThreads, total - 1);
-      m[u] = item / pairs;
-      j[u] = 2 * (item - m[u] * pairs);
-      const int n = n0 + j[u];
-      const bool second = n + 1 < e.N;
-      ws[u] = make_float2(e.w_scale[n], second ? e.w_scale[n + 1] : 0.f);
-      b[u] = e.bias != nullptr ? make_float2(e.bias[n], second ? e.bias[n + 1] : 0.f) : make_float2(0.f, 0.f);
-      r[u] = make_float2(0.f, 0.f);
-      if (KIND != GATED && e.residual != nullptr && base + u * kThreads < total) {
-        const float* from = e.residual + (m0 + m[u]) * e.residual_stride + n;
-        r[u] = make_float2(from[0], second ? from[1] : 0.f);
-      }
-      sum[u] = make_float2(0.f, 0.f);
+      m[u] = item / quads;
+      j[u] = 4 * (item - m[u] * quads);
+      const int n = n0 + j[u], last = e.N - 1;
+      ws[u] = make_float4(e.w_scale[n], e.w_scale[min(n + 1, last)], e.w_scale[min(n + 2, last)], e.w_scale[min(n + 3, last)]);
+      b[u] = r[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (e.bias != nullptr) b[u] = make_float4(e.bias[n], e.bias[min(n + 1, last)], e.bias[min(n + 2, last)], e.bias[min(n + 3, last)]);
+      if (KIND != GATED && e.residual != nullptr && base + u * kThreads < total) r[u] = residual_quad(e, m0 + m[u], n);
+      sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     for (int member = 0; member < members; ++member) {
 #pragma unroll
       for (int u = 0; u < kItems; ++u) {
-        const float2 part = *reinterpret_cast<const float2*>(inbox + member * plane + m[u] * slice + j[u]);
-        sum[u].x += part.x;
-        sum[u].y += part.y;
+        const float4 part = *reinterpret_cast<const float4*>(inbox + member * plane + m[u] * slice + j[u]);
+        sum[u] = make_float4(sum[u].x + part.x, sum[u].y + part.y, sum[u].z + part.z, sum[u].w + part.w);
       }
     }
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
       if (base + u * kThreads >= total) break;
       const float xs = x_scales[m[u]];
+      float4 v = make_float4(fmaf(sum[u].x * xs, ws[u].x, b[u].x), fmaf(sum[u].y * xs, ws[u].y, b[u].y), fmaf(sum[u].z * xs, ws[u].z, b[u].z),
+                                   fmaf(sum[u].w * xs, ws[u].w, b[u].w));
       const int n = n0 + j[u];
-      float v[2] = {fmaf(sum[u].x * xs, ws[u].x, b[u].x), fmaf(sum[u].y * xs, ws[u].y, b[u].y)};
-      T* to = static_cast<T*>(e.out) + (m0 + m[u]) * e.out_stride;
-      if constexpr (KIND == GATED) {
-        to[n >> 1] = from_f32<T>(e.activation == ACT_GELU ? gated_unit<true>(v[0], v[1]) : gated_unit<false>(v[0], v[1]));
-      } else {
-        if constexpr (KIND == ACTIVATED) activate_all<2>(v, e.activation);
-        v[0] += r[u].x;
-        v[1] += r[u].y;
-        if (e.pairs) {
-          if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to + n) = make_float2(v[0], v[1]);
-          else *reinterpret_cast<__nv_bfloat162*>(to + n) = __floats2bfloat162_rn(v[0], v[1]);
-        } else {
-          to[n] = from_f32<T>(v[0]);
-          if (n + 1 < e.N) to[n + 1] = from_f32<T>(v[1]);
-        }
-      }
+      if constexpr (KIND == ACTIVATED) v = activate_quad(v, e.activation);
+      if constexpr (KIND != GATED) v = add_each(v, r[u]);
+      T* to = static_cast<T*>(e.out) + (m0 + m[u]) * e.out_stride + (KIND == GATED ? n >> 1 : n);
+      if (e.vector && n + 3 < e.N) store_whole<KIND, T>(to, v, e.activation);
+      else store_some<KIND, T>(to, n, e.N, v, e.activation);
     }
   }
 }
@@ -129,6 +115,7 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   __shared__ __align__(8) uint64_t accum_bar;
   __shared__ uint32_t tmem_base_shared;
   __shared__ __align__(16) float x_scales[kMaxTokens];
+  __shared__ __align__(16) float stages_out[CLUSTERED ? 4 : 4 * kStageFloats];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int stages = p.stages;
@@ -226,21 +213,16 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31 belong to this warp
   const int row = quarter * 32 + lane;
   if (warp >= 2) {
-    const int n = n0 + row;
-    float ws = 0.f, b = 0.f;
-    if (!CLUSTERED && n < p.e.N) {
-      ws = p.e.w_scale[n];
-      if (p.e.bias != nullptr) b = p.e.bias[n];
-    }
     const bool have = mbar_wait(&accum_bar, 0);
     if (!have && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if constexpr (!CLUSTERED) {
       const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
-      for (int c0 = 0; have && c0 < tokens; c0 += 16) {
-        float v[16];
-        tmem_sums_16(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, chains, p.tile, v);
-        finish_columns<KIND, T, 16>(p.e, x_scales + c0, ws, b, m0 + c0, n, v);
+      WayOut<KIND, T> way(p.e, m0, n0 + quarter * 32, stages_out + (warp - 2) * kStageFloats);
+      for (int c0 = 0; have && c0 < tokens; c0 += 8) {
+        float v[8];
+        tmem_sums(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, chains, p.tile, v);
+        way.take(x_scales + c0, v);
       }
     }
   }
@@ -250,11 +232,11 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
       const int owner = row / slice;
       const uint32_t mine = peer_address(inbox + static_cast<int64_t>(rank) * tokens * slice + (row - owner * slice), owner);
-      for (int c0 = 0; c0 < tokens; c0 += 16) {
-        float v[16];
-        tmem_sums_16(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, chains, p.tile, v);
+      for (int c0 = 0; c0 < tokens; c0 += 8) {
+        float v[8];
+        tmem_sums(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, chains, p.tile, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 8; ++i)
           if (c0 + i < tokens) store_peer_f32(mine + static_cast<uint32_t>((c0 + i) * slice) * sizeof(float), v[i]);
       }
     }

@@ -4,11 +4,11 @@
 // The two blocks of a cluster are one `tcgen05.mma.cta_group::2` (kind::f8f6f4): each holds 128 of the tile's rows of W and half of its tokens in
 // shared memory and 128 rows of the sums in TMEM, so what an SM takes out of L2 for 128 k is 16 KB of W and 16 KB of X for 128 x 256 sums, where a
 // block by itself would need 48. Persistent: a cluster per two SMs walks over the tiles. In each block one thread fills a ring of stages by TMA
-// (both blocks' copies are counted on the leader's barriers), in the leader one thread issues the products, and eight warps per block read the
-// sums of one tile while the next is made in the other half of TMEM. A lane has one row of W and half of the tile's tokens: scales and bias of
-// the row are the lane's own, and a warp stores 32 neighbours of an output row (finish_columns in float8.cuh).
+// (both blocks' copies are counted on the leader's barriers), in the leader one thread issues the products, and sixteen warps per block read the
+// sums of one tile while the next is made in the other half of TMEM. A lane has one row of W and a quarter of the tile's tokens: scales and bias of
+// the row are the lane's own; on their way out the numbers change places inside a warp (WayOut in float8.cuh).
 //
-// 32-bit outputs: after each chain of kChainBlocks k-blocks the eight warps add the sums to registers and the products go on in the other half.
+// 32-bit outputs: after each chain of kChainBlocks k-blocks the warps add the sums to registers and the products go on in the other half.
 //
 // Tiles are taken in strips of a few token tiles across all rows of W, so that at any time the clusters share a few rows of both operands in L2.
 // TMEM (all of it) is taken after the kernel in front has ended, shared memory leaves no room for another block. Every wait is bounded: a role that
@@ -20,8 +20,8 @@ namespace {
 
 constexpr int kPairRows = 2 * kRowsW;     // rows of W of a tile: MMA M
 constexpr int kMostTokens = 256;          // tokens of a tile: MMA N, a multiple of 32
-constexpr int kSumWarps = 8;
-constexpr int kThreads = (2 + kSumWarps) * 32;  // warp 0: TMA, warp 1: MMA, 2-9: sums
+constexpr int kSumWarps = 16;                   // four a quarter of the TMEM lanes
+constexpr int kThreads = (2 + kSumWarps) * 32;  // warp 0: TMA, warp 1: MMA, 2-17: sums
 constexpr int kMaxStages = 10;
 constexpr int kStrip = 8;                 // token tiles of a strip
 constexpr size_t kRingBytes = 6 * 32 * 1024;
@@ -60,8 +60,9 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
                "h"(static_cast<uint16_t>(3))
                : "memory");
 }
+// What it says is that TMEM has been read (tcgen05.wait::ld has returned); with release it would wait for all stores of the warp, 1,000 cycles.
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
 // Tile `at` of the order described above: its token tile and its rows-of-W tile.
@@ -88,6 +89,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   __shared__ __align__(8) uint64_t sums_empty[2];
   __shared__ uint32_t tmem_base_shared;
   __shared__ __align__(16) float x_scales[2][kMostTokens];
+  __shared__ __align__(16) float stages_out[kSumWarps * kStageFloats];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x & 1;
@@ -194,88 +196,77 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
     }
   } else {
     const int quarter = warp & 3;             // TMEM lanes 32 * quarter .. + 31 belong to this warp
-    const int side = (warp - 2) >> 2;         // which half of the tokens
-    const int width = p.tile / 2;             // a multiple of 16
+    const int side = (warp - 2) >> 2;         // which quarter of the tokens
+    const int width = p.tile / 4;             // a multiple of 8
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + side * width;
     const uint32_t leader_empty = of_leader(sums_empty);
     const int tid = threadIdx.x - 64;
+    float* stage = stages_out + (warp - 2) * kStageFloats;
     int item = 0;
     bool alive = true;
     for (int at = cluster, turn = 0; at < total; at += clusters, turn ^= 1) {  // to the end even after giving up: the warps meet once a tile
       int tm, tn;
       locate(at, tiles_m, tiles_n, tm, tn);
       const int m0 = tm * p.tile;
-      const int n = tn * kPairRows + rank * kRowsW + quarter * 32 + lane;
-      // The tile's token scales, for all eight warps; the copy of two tiles ago is read by nobody any more (a warp meets the others once a tile).
+      const int n0 = tn * kPairRows + rank * kRowsW + quarter * 32;
+      // The tile's token scales, for all warps; the copy of two tiles ago is read by nobody any more (a warp meets the others once a tile).
       if (tid < p.tile) x_scales[turn][tid] = m0 + tid < p.e.M ? p.e.x_scale[m0 + tid] : 0.f;
-      float ws = 0.f, b = 0.f;
-      if (n < p.e.N) {
-        ws = p.e.w_scale[n];
-        if (p.e.bias != nullptr) b = p.e.bias[n];
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
       const float* xs = x_scales[turn] + side * width;
-      if constexpr (!kChained) {
-        const int half = item & 1;
-        alive = alive && mbar_wait(&sums_full[half], (item >> 1) & 1);
-        if (alive) {
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          // Two sets of registers: the next 16 columns are on their way while these are finished.
-          const uint32_t from = lanes + half * kMostTokens;
-          float v[2][16];
-          tmem_ask_16(from, v[0]);
-          tmem_wait(v[0]);
-          for (int c = 0; c < width; c += 32) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int now = c + u * 16;
-              if (now < width) {
-                if (now + 16 < width) {
-                  tmem_ask_16(from + now + 16, v[u ^ 1]);
-                } else {  // the last of it is in registers: the products of the tile after next may begin
-                  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                  __syncwarp();
-                  if (lane == 0) arrive_at(leader_empty + half * 8);
-                }
-                finish_columns<KIND, T, 16>(p.e, xs + now, ws, b, m0 + side * width + now, n, v[u]);
-                if (now + 16 < width) tmem_wait(v[u ^ 1]);
-              }
-            }
-          }
+      // Waits for a tile's (or a chain's) sums and says where in TMEM they are.
+      auto sums_of = [&](int which) {
+        alive = alive && mbar_wait(&sums_full[which & 1], (which >> 1) & 1);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return lanes + (which & 1) * kMostTokens;
+      };
+      auto sums_read = [&](int which) {  // they are in registers: the products after next may go there
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive_at(leader_empty + (which & 1) * 8);
+      };
+      auto finish = [&](WayOut<KIND, T>& way, uint32_t from) {
+        for (int c = 0; c < width; c += 8) {
+          float v[8];
+          tmem_ask(from + c, v);
+          tmem_wait(v);
+          if (c + 8 >= width) sums_read(item);
+          way.take(xs + c, v);
         }
+      };
+      if constexpr (!kChained) {
+        WayOut<KIND, T> way(p.e, m0 + side * width, n0, stage);
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+        const uint32_t from = sums_of(item);
+        if (alive) finish(way, from);
         ++item;
       } else {
-        float acc[kMostTokens / 32][16];
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+        uint32_t from = lanes;
+        if (links > 1) {  // the chains in registers; with the last one back to where that lies
+          float acc[kMostTokens / 32][8];
+          for (int link = 0; link < links; ++link) {
+            from = sums_of(item + link);
+            if (!alive) break;
 #pragma unroll
-        for (int g = 0; g < kMostTokens / 32; ++g)
+            for (int g = 0; g < kMostTokens / 32; ++g) {
+              if (g * 8 < width) {
+                float v[8];
+                tmem_ask(from + g * 8, v);
+                tmem_wait(v);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[g][i] = 0.f;
-        for (int link = 0; link < links && alive; ++link, ++item) {
-          const int half = item & 1;
-          if (!mbar_wait(&sums_full[half], (item >> 1) & 1)) {
-            alive = false;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-          for (int g = 0; g < kMostTokens / 32; ++g) {
-            if (g * 16 < width) {
-              float v[16];
-              tmem_ask_16(lanes + half * kMostTokens + g * 16, v);
-              tmem_wait(v);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) acc[g][i] += v[i];
+                for (int i = 0; i < 8; ++i) acc[g][i] = link > 0 ? acc[g][i] + v[i] : v[i];
+                if (link == links - 1) tmem_store(from + g * 8, acc[g]);
+              }
             }
+            if (link < links - 1) sums_read(item + link);
           }
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) arrive_at(leader_empty + half * 8);
+          tmem_stored();
+          item += links - 1;
+        } else {
+          from = sums_of(item);
         }
-        if (alive) {
-#pragma unroll
-          for (int g = 0; g < kMostTokens / 32; ++g)
-            if (g * 16 < width) finish_columns<KIND, T, 16>(p.e, xs + g * 16, ws, b, m0 + side * width + g * 16, n, acc[g]);
-        }
+        WayOut<KIND, T> way(p.e, m0 + side * width, n0, stage);
+        if (alive) finish(way, from);
+        ++item;
       }
     }
     if (!alive && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
