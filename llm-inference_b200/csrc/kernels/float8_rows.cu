@@ -245,34 +245,59 @@ int launch_rows(const RowsParams& p, bool packs, int dtype, cudaStream_t stream)
 }  // namespace
 }  // namespace float8
 
-// Strides in elements. dtype: of x.
-B200_API int b200_float8_quantize(const void* x, int dtype, int64_t x_stride, void* out, int64_t out_stride, float* scales, int rows, int columns,
-                                  cudaStream_t stream) {
+// The numbers of a call, in the order in which parts/float8.py packs them; pitches in elements.
+struct Float8Quantize {
+  const void* x;
+  int64_t dtype, x_pitch;  // dtype: of x
+  void* out;
+  int64_t out_pitch;
+  float* scales;
+  int64_t rows, columns;
+};
+struct Float8RmsNorm {
+  const float* x;
+  int64_t x_pitch;
+  const void* delta;
+  int64_t dtype, delta_pitch;  // dtype: of delta (of nothing where there is none)
+  const float* weight;
+  float* stream;
+  int64_t stream_pitch;
+  void* out;
+  int64_t out_pitch;
+  float* scales;
+  int64_t rows, columns;
+  double eps;
+};
+static_assert(sizeof(Float8Quantize) == 8 * 8 && sizeof(Float8RmsNorm) == 14 * 8, "as packed by the caller");
+
+static bool float8_sizes(int64_t rows, int64_t columns) { return rows > 0 && columns > 0 && rows < (int64_t(1) << 31) && columns < (int64_t(1) << 31); }
+
+B200_API int b200_float8_quantize(const Float8Quantize* c, cudaStream_t stream) {
   using namespace float8;
-  if (rows == 0) return 0;
-  B200_REQUIRE(rows > 0 && columns > 0, "float8 quantize: bad sizes");
-  B200_REQUIRE(dtype == DTYPE_F32 || dtype == DTYPE_BF16, "float8 quantize: unknown dtype %d", dtype);
+  if (c->rows == 0) return 0;
+  B200_REQUIRE(float8_sizes(c->rows, c->columns), "float8 quantize: bad sizes");
+  B200_REQUIRE(c->dtype == DTYPE_F32 || c->dtype == DTYPE_BF16, "float8 quantize: unknown dtype %d", static_cast<int>(c->dtype));
   RowsParams p = {};
-  p.x = x, p.x_stride = x_stride, p.out = static_cast<uint8_t*>(out), p.out_stride = out_stride, p.scales = scales, p.rows = rows, p.columns = columns;
-  const int size = dtype == DTYPE_F32 ? 4 : 2;
-  const bool packs = columns % 8 == 0 && aligned(x, x_stride * size, 16) && aligned(out, out_stride, 8);
-  return launch_rows<false>(p, packs, dtype, stream);
+  p.x = c->x, p.x_stride = c->x_pitch, p.out = static_cast<uint8_t*>(c->out), p.out_stride = c->out_pitch, p.scales = c->scales;
+  p.rows = static_cast<int>(c->rows), p.columns = static_cast<int>(c->columns);
+  const int size = c->dtype == DTYPE_F32 ? 4 : 2;
+  const bool packs = p.columns % 8 == 0 && aligned(c->x, c->x_pitch * size, 16) && aligned(c->out, c->out_pitch, 8);
+  return launch_rows<false>(p, packs, static_cast<int>(c->dtype), stream);
 }
 
-// dtype: of delta (of nothing where there is none).
-B200_API int b200_float8_rmsnorm(const float* x, int64_t x_stride, const void* delta, int dtype, int64_t delta_stride, const float* weight, float eps,
-                                 float* stream_out, int64_t stream_stride, void* out, int64_t out_stride, float* scales, int rows, int columns,
-                                 cudaStream_t stream) {
+B200_API int b200_float8_rmsnorm(const Float8RmsNorm* c, cudaStream_t stream) {
   using namespace float8;
-  if (rows == 0) return 0;
-  B200_REQUIRE(rows > 0 && columns > 0, "float8 rmsnorm: bad sizes");
-  B200_REQUIRE(dtype == DTYPE_F32 || dtype == DTYPE_BF16, "float8 rmsnorm: unknown dtype %d", dtype);
+  if (c->rows == 0) return 0;
+  B200_REQUIRE(float8_sizes(c->rows, c->columns), "float8 rmsnorm: bad sizes");
+  B200_REQUIRE(c->dtype == DTYPE_F32 || c->dtype == DTYPE_BF16, "float8 rmsnorm: unknown dtype %d", static_cast<int>(c->dtype));
   RowsParams p = {};
-  p.x = x, p.x_stride = x_stride, p.delta = delta, p.delta_stride = delta_stride, p.weight = weight, p.eps = eps;
-  p.stream = stream_out, p.stream_stride = stream_stride;
-  p.out = static_cast<uint8_t*>(out), p.out_stride = out_stride, p.scales = scales, p.rows = rows, p.columns = columns;
-  const int size = dtype == DTYPE_F32 ? 4 : 2;
-  const bool packs = columns % 8 == 0 && aligned(x, x_stride * 4, 16) && aligned(weight, 0, 16) && aligned(out, out_stride, 8) &&
-                     (delta == nullptr || aligned(delta, delta_stride * size, 16)) && (stream_out == nullptr || aligned(stream_out, stream_stride * 4, 16));
-  return launch_rows<true>(p, packs, dtype, stream);
+  p.x = c->x, p.x_stride = c->x_pitch, p.delta = c->delta, p.delta_stride = c->delta_pitch, p.weight = c->weight, p.eps = static_cast<float>(c->eps);
+  p.stream = c->stream, p.stream_stride = c->stream_pitch;
+  p.out = static_cast<uint8_t*>(c->out), p.out_stride = c->out_pitch, p.scales = c->scales;
+  p.rows = static_cast<int>(c->rows), p.columns = static_cast<int>(c->columns);
+  const int size = c->dtype == DTYPE_F32 ? 4 : 2;
+  const bool packs = p.columns % 8 == 0 && aligned(c->x, c->x_pitch * 4, 16) && aligned(c->weight, 0, 16) && aligned(c->out, c->out_pitch, 8) &&
+                     (c->delta == nullptr || aligned(c->delta, c->delta_pitch * size, 16)) &&
+                     (c->stream == nullptr || aligned(c->stream, c->stream_pitch * 4, 16));
+  return launch_rows<true>(p, packs, static_cast<int>(c->dtype), stream);
 }

@@ -35,29 +35,49 @@ int make_map(CUtensorMap* map, const void* base, int rows, int K, int64_t stride
 
 }  // namespace float8
 
-// y = epilogue(x w^T): x [M, K] and w [N, K] in e4m3 (strides in bytes, multiples of 16), scales a row each. kind: 0 plain, 1 activated, 2 gated
-// (W's rows in pairs; out has N / 2 columns, no residual). out and residual strides in elements.
-B200_API int b200_float8_linear(const void* x, int64_t x_stride, const float* x_scale, const void* w, int64_t w_stride, const float* w_scale, int w_constant,
-                                void* out, int out_dtype, int64_t out_stride, const float* bias, const float* residual, int64_t residual_stride, int M, int N,
-                                int K, int kind, int activation, int* err, cudaStream_t stream) {
+// The numbers of a call, in the order in which parts/float8.py packs them: y = epilogue(x w^T), x [M, K] and w [N, K] in e4m3 (pitches in bytes, multiples
+// of 16), scales a row each. kind: 0 plain, 1 activated, 2 gated (W's rows in pairs; out has N / 2 columns, no residual). out and residual pitches in elements.
+struct Float8Linear {
+  const void* x;
+  int64_t x_pitch;
+  const float* x_scales;
+  const void* w;
+  int64_t w_pitch;
+  const float* w_scales;
+  int64_t w_constant;
+  void* out;
+  int64_t out_dtype, out_pitch;
+  const float* bias;
+  const float* residual;
+  int64_t residual_pitch, M, N, K, kind, activation;
+  int* err;
+};
+static_assert(sizeof(Float8Linear) == 19 * 8, "as packed by the caller");
+
+B200_API int b200_float8_linear(const Float8Linear* c, cudaStream_t stream) {
   using namespace float8;
-  if (M == 0 || N == 0) return 0;
-  B200_REQUIRE(M > 0 && N > 0 && K > 0, "float8 product: bad sizes %d x %d x %d", M, N, K);
-  B200_REQUIRE(kind >= PLAIN && kind <= GATED, "float8 product: unknown kind %d", kind);
-  B200_REQUIRE(activation >= ACT_NONE && activation <= ACT_SQUARED_RELU && (kind == PLAIN) == (activation == ACT_NONE), "float8 product: unknown activation %d",
-               activation);
-  B200_REQUIRE(kind != GATED || (N % 2 == 0 && activation != ACT_SQUARED_RELU && residual == nullptr), "float8 product: the gated form takes pairs of rows, silu or gelu, no residual");
-  B200_REQUIRE(out_dtype == DTYPE_F32 || out_dtype == DTYPE_BF16, "float8 product: unknown dtype %d", out_dtype);
-  B200_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 && x_stride % 16 == 0 && w_stride % 16 == 0 && x_stride >= K &&
-                   w_stride >= K,
-               "float8 product: operands' rows start on 16-byte boundaries");
+  if (c->M == 0 || c->N == 0) return 0;
+  constexpr int64_t kMost = (int64_t(1) << 31) - 1;
+  B200_REQUIRE(c->M > 0 && c->N > 0 && c->K > 0 && c->M <= kMost && c->N <= kMost && c->K <= kMost, "float8 product: bad sizes");
   Product p;
-  p.x = x, p.w = w, p.x_stride = x_stride, p.w_stride = w_stride, p.K = K, p.kind = kind, p.out_f32 = out_dtype == DTYPE_F32, p.w_constant = w_constant, p.err = err;
-  p.e.out = out, p.e.x_scale = x_scale, p.e.w_scale = w_scale, p.e.bias = bias, p.e.residual = residual;
-  p.e.out_stride = out_stride, p.e.residual_stride = residual_stride, p.e.M = M, p.e.N = N, p.e.activation = activation;
-  const int size = out_dtype == DTYPE_F32 ? 4 : 2, at_once = kind == GATED ? 2 : 4;  // outputs from four rows of W
-  p.e.vector = out_stride % at_once == 0 && reinterpret_cast<uintptr_t>(out) % (at_once * size) == 0 &&
-               (residual == nullptr || (residual_stride % 4 == 0 && reinterpret_cast<uintptr_t>(residual) % 16 == 0));
+  p.x = c->x, p.w = c->w, p.x_stride = c->x_pitch, p.w_stride = c->w_pitch, p.K = static_cast<int>(c->K);
+  p.kind = static_cast<int>(c->kind), p.out_f32 = c->out_dtype == DTYPE_F32, p.w_constant = c->w_constant != 0, p.err = c->err;
+  Epilogue& e = p.e;
+  e.out = c->out, e.x_scale = c->x_scales, e.w_scale = c->w_scales, e.bias = c->bias, e.residual = c->residual;
+  e.out_stride = c->out_pitch, e.residual_stride = c->residual_pitch, e.M = static_cast<int>(c->M), e.N = static_cast<int>(c->N);
+  e.activation = static_cast<int>(c->activation);
+  B200_REQUIRE(p.kind >= PLAIN && p.kind <= GATED, "float8 product: unknown kind %d", p.kind);
+  B200_REQUIRE(e.activation >= ACT_NONE && e.activation <= ACT_SQUARED_RELU && (p.kind == PLAIN) == (e.activation == ACT_NONE),
+               "float8 product: unknown activation %d", e.activation);
+  B200_REQUIRE(p.kind != GATED || (e.N % 2 == 0 && e.activation != ACT_SQUARED_RELU && e.residual == nullptr),
+               "float8 product: the gated form takes pairs of rows, silu or gelu, no residual");
+  B200_REQUIRE(c->out_dtype == DTYPE_F32 || c->out_dtype == DTYPE_BF16, "float8 product: unknown dtype %d", static_cast<int>(c->out_dtype));
+  B200_REQUIRE(reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0 && p.x_stride % 16 == 0 && p.w_stride % 16 == 0 &&
+                   p.x_stride >= p.K && p.w_stride >= p.K,
+               "float8 product: operands' rows start on 16-byte boundaries");
+  const int size = p.out_f32 ? 4 : 2, at_once = p.kind == GATED ? 2 : 4;  // outputs from four rows of W
+  e.vector = e.out_stride % at_once == 0 && reinterpret_cast<uintptr_t>(e.out) % (at_once * size) == 0 &&
+             (e.residual == nullptr || (e.residual_stride % 4 == 0 && reinterpret_cast<uintptr_t>(e.residual) % 16 == 0));
   if (float8::g_tile > 0) return launch_tiles(p, float8::g_tile, stream);
   return launch_stream(p, stream);
 }

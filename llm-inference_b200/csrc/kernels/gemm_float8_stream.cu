@@ -1,13 +1,13 @@
 // Product of 8-bit rows for few tokens: the weights stream past the tensor cores once, K split inside thread-block clusters.
 //   y[m][n] = act((sum_k x[m][k] w[n][k]) xs[m] ws[n] + bias[n]) + residual[m][n],  or act(gate) * up over pairs of W's rows.
 //
-// W is the wide operand: a block owns 128 rows of W (the MMA's M) and a tile of up to 256 tokens (its N, a multiple of 16). One thread fills a ring
+// W is the wide operand: a block owns 128 rows of W (the MMA's M) and a tile of up to 128 tokens (its N, a multiple of 16). One thread fills a ring
 // of stages by TMA (128 rows x 128 bytes of W, tokens x 128 bytes of X, 128-byte swizzle), one issues `tcgen05.mma` (kind::f8f6f4, 32 k an
 // instruction) into TMEM, four warps read the sums back, a lane per row of W. Where W has too few rows to give every SM work, the blocks of a
-// cluster share rows and split K: each pushes its partial sums into the shared memory of the member that finishes those rows, the cluster meets,
-// and the owners add in member order, so a sum does not depend on timing. With up to 16 tokens the inboxes lie behind the ring and the
-// cluster meets once; with more they take the ring's place, so it meets before the push too (stores into a neighbour's memory need no answer, loads
-// out of it wait for one).
+// cluster share rows and split K: each sends its partial sums to the shared memory of the member that finishes those rows, and the owners add in
+// member order, so a sum does not depend on timing. With up to 16 tokens the inboxes lie behind the ring, the sums are stored there from registers
+// and the cluster meets once. With more tokens outbox and inbox take the ring's place, so the cluster meets first; a slice then travels as
+// one bulk copy to its owner, who waits for the bytes (64 tokens of 4,608 x 3,584: single stores 9.9 us, copies TIME_BULK).
 //
 // 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as TMEM goes, added up as they are read.
 //
@@ -27,7 +27,7 @@ constexpr int kThreads = 192;      // warp 0: TMA, warp 1: MMA, warps 2-5: sums
 constexpr int kMaxStages = 12;
 constexpr int kMaxMembers = 16;
 constexpr int kEarlyTokens = 16;   // up to this many (padded) tokens the inboxes lie behind the ring
-constexpr int kMaxTokens = 256;    // a block's
+constexpr int kMaxTokens = 128;    // a block's
 
 struct StreamParams {
   Epilogue e;
@@ -54,6 +54,18 @@ __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t a_desc, uint64_t 
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// Bytes of the outbox: a slice per owner, of the padded tokens.
+__host__ __device__ constexpr size_t outbox_bytes(int members, int tile) {
+  const int slice = slice_rows(members), owners = (kRowsW + slice - 1) / slice;
+  return static_cast<size_t>(owners) * slice * tile * sizeof(float);
+}
+// `bytes` (a multiple of 16) from here to the same place of block `rank`, counted on that block's barrier.
+__device__ __forceinline__ void copy_to_peer(float* dst, const float* src, uint32_t bytes, uint64_t* bar, int rank) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(peer_address(dst, rank)), "r"(smem_addr(src)),
+               "r"(bytes), "r"(peer_address(bar, rank))
+               : "memory");
 }
 
 // What one member finishes: `rows` rows of W from n0 on, the members' partial sums ([members][tokens][slice]) added in member order. An item is four
@@ -113,6 +125,7 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   __shared__ __align__(8) uint64_t full_bar[kMaxStages];
   __shared__ __align__(8) uint64_t empty_bar[kMaxStages];
   __shared__ __align__(8) uint64_t accum_bar;
+  __shared__ __align__(8) uint64_t inbox_bar;
   __shared__ uint32_t tmem_base_shared;
   __shared__ __align__(16) float x_scales[kMaxTokens];
   __shared__ __align__(16) float stages_out[CLUSTERED ? 4 : 4 * kStageFloats];
@@ -136,6 +149,7 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       mbar_init(&empty_bar[s], 1);
     }
     mbar_init(&accum_bar, 1);
+    mbar_init(&inbox_bar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     // The thread that made the barriers also loads: the first weights are on their way before the block has met.
     if (!p.w_constant) wait_for_predecessor();
@@ -205,10 +219,6 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   }
   __syncwarp();
 
-  const int slice = slice_rows(members);
-  const bool early = p.tile <= kEarlyTokens;
-  // [members][tokens][slice] partial sums, behind the ring or (once every member is done with its products) in its place.
-  float* inbox = reinterpret_cast<float*>(tiles + (early ? static_cast<size_t>(stages) * stage_bytes : 0));
   const int tokens = min(p.tile, p.e.M - m0);
   const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31 belong to this warp
   const int row = quarter * 32 + lane;
@@ -227,21 +237,48 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     }
   }
   if constexpr (CLUSTERED) {
-    if (!early) cluster_sync_all();  // nobody's ring is read any more
-    if (warp >= 2) {
-      const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
-      const int owner = row / slice;
-      const uint32_t mine = peer_address(inbox + static_cast<int64_t>(rank) * tokens * slice + (row - owner * slice), owner);
-      for (int c0 = 0; c0 < tokens; c0 += 8) {
-        float v[8];
-        tmem_sums(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, chains, p.tile, v);
+    const int slice = slice_rows(members);
+    const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
+    const bool early = p.tile <= kEarlyTokens;
+    const int plane = tokens * slice;  // what one member sends to one owner: [tokens][slice]
+    const int owner = row / slice, in_slice = row - owner * slice;
+    const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    float* inbox = reinterpret_cast<float*>(tiles + (early ? static_cast<size_t>(stages) * stage_bytes : outbox_bytes(members, p.tile)));  // [members][plane]
+    if (early) {
+      if (warp >= 2) {
+        const uint32_t mine = peer_address(inbox + rank * plane + in_slice, owner);
+        for (int c0 = 0; c0 < tokens; c0 += 8) {
+          float v[8];
+          tmem_sums(lanes + c0, chains, p.tile, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c0 + i < tokens) store_peer_f32(mine + static_cast<uint32_t>((c0 + i) * slice) * sizeof(float), v[i]);
+          for (int i = 0; i < 8; ++i)
+            if (c0 + i < tokens) store_peer_f32(mine + static_cast<uint32_t>((c0 + i) * slice) * sizeof(float), v[i]);
+        }
       }
+      cluster_sync_all();
+    } else {
+      float* outbox = reinterpret_cast<float*>(tiles);  // [owners][plane]
+      cluster_sync_all();  // nobody's ring is read any more
+      if (warp >= 2) {
+        float* mine = outbox + owner * plane + in_slice;
+        for (int c0 = 0; c0 < tokens; c0 += 8) {
+          float v[8];
+          tmem_sums(lanes + c0, chains, p.tile, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c0 + i < tokens) mine[(c0 + i) * slice] = v[i];
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const uint32_t bytes = static_cast<uint32_t>(plane) * sizeof(float);
+        if (threadIdx.x == 64 && rank * slice < kRowsW) mbar_expect_tx(&inbox_bar, members * bytes);
+        const int to = threadIdx.x - 64;  // a thread per owner
+        if (to < members && to * slice < kRowsW) copy_to_peer(inbox + rank * plane, outbox + to * plane, bytes, &inbox_bar, to);
+      }
+      if (rank * slice < kRowsW && !mbar_wait(&inbox_bar, 0) && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
     }
-    cluster_sync_all();
     finish_slice<KIND, T>(p.e, inbox, x_scales, m0, tokens, n0 + rank * slice, max(0, min(kRowsW - rank * slice, slice)), slice, members);
+    if (!early) cluster_sync_all();  // nobody's outbox is read any more
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -320,7 +357,7 @@ void size_ring(StreamPlan& plan, int k_blocks, bool f32) {
   const int per_block = (k_blocks + plan.members - 1) / plan.members;
   // Accumulators: one, or one per chain where outputs are 32-bit, as many as fit.
   const int wanted = f32 ? (per_block + kChainBlocks - 1) / kChainBlocks : 1;
-  const bool alone = plan.tile > 128 || (wanted > 1 && wanted * plan.tile > 128 && plan.tile > 16);  // more than a quarter of TMEM: the SM to itself
+  const bool alone = wanted > 1 && wanted * plan.tile > 128 && plan.tile > 16;  // more than a quarter of TMEM: the SM to itself
   const int most = alone ? 256 : 128;
   const int accumulators = max(1, min(wanted, most / plan.tile));
   plan.chain_blocks = (per_block + accumulators - 1) / accumulators;
@@ -334,7 +371,7 @@ void size_ring(StreamPlan& plan, int k_blocks, bool f32) {
   plan.stages = max(stages, 2);
   const size_t ring = plan.stages * stage;
   const size_t inbox = plan.members > 1 ? static_cast<size_t>(plan.members) * slice_rows(plan.members) * plan.tile * sizeof(float) : 0;
-  plan.smem = (plan.tile <= kEarlyTokens ? ring + inbox : max(ring, inbox)) + 1024;
+  plan.smem = (plan.tile <= kEarlyTokens ? ring + inbox : max(ring, inbox > 0 ? outbox_bytes(plan.members, plan.tile) + inbox : 0)) + 1024;
   if (alone) plan.smem = max(plan.smem, static_cast<size_t>(118 * 1024));  // TMEM goes with shared memory: see the head of the file
   else plan.smem = max(plan.smem, static_cast<size_t>(plan.tmem_cols) * 227 * 1024 / 512);
 }
@@ -342,8 +379,7 @@ void size_ring(StreamPlan& plan, int k_blocks, bool f32) {
 StreamPlan plan_uncached(int M, int N, int K, bool f32) {
   StreamPlan plan;
   plan.blocks = (N + kRowsW - 1) / kRowsW;
-  const int most = f32 ? 128 : kMaxTokens;
-  plan.tiles = (M + most - 1) / most;
+  plan.tiles = (M + kMaxTokens - 1) / kMaxTokens;
   plan.tile = (((M + plan.tiles - 1) / plan.tiles) + 15) / 16 * 16;
   const int k_blocks = (K + kBlockK - 1) / kBlockK;
   const int sms = b200_sm_count_host();

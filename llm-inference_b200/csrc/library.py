@@ -8,7 +8,7 @@ and loaded from the source tree. There is no fallback: if it cannot be built or 
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 from functools import lru_cache
 
 import torch
@@ -50,10 +50,9 @@ def stream_handle() -> c_void_p:
 _SIGNATURES: dict[str, list] = {
     "b200_embedding_gather": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p],
     "b200_rmsnorm": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_void_p],
-    "b200_float8_quantize": [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p],
-    "b200_float8_rmsnorm": [c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p],
-    "b200_float8_linear": [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64]
-    + [c_int] * 5 + [c_void_p, c_void_p],
+    "b200_float8_quantize": [c_char_p, c_void_p],  # the numbers of a call as one block, see parts/float8.py
+    "b200_float8_rmsnorm": [c_char_p, c_void_p],
+    "b200_float8_linear": [c_char_p, c_void_p],
     "b200_silu_mul": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "b200_gelu_mul": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "b200_rope_kv_write": [c_void_p] * 7 + [c_int, c_int] + [c_void_p] * 3 + [c_int] * 8 + [c_void_p, c_void_p],

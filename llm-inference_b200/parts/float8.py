@@ -8,12 +8,12 @@ stream of the step's device and writes into tensors that it is handed. The kerne
 
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_int64
 from dataclasses import dataclass
+from struct import Struct
 
 import torch
 
-from ..csrc.library import DTYPE_CODES, KernelError, ptr
+from ..csrc.library import DTYPE_CODES, KernelError
 from .context import StepContext
 
 LARGEST = 448.0  # of e4m3
@@ -37,12 +37,6 @@ class Float8Rows:
     @property
     def shape(self) -> tuple[int, int]:
         return tuple(self.values.shape)
-
-    @property
-    def row_stride(self) -> int:
-        """Bytes from row to row (of a single row: what they would be)."""
-        rows, columns = self.values.shape
-        return self.values.stride(0) if rows > 1 else -(-columns // ROW_BYTES) * ROW_BYTES
 
     def bytes(self) -> int:
         return self.values.numel() + 4 * self.scales.numel()
@@ -84,51 +78,85 @@ def _need(cond: bool, message: str) -> None:
         raise KernelError(message)
 
 
-def _need_rows(name: str, m: Float8Rows, device: torch.device) -> None:
+# Operands are checked with as few trips into the tensor library as it takes: a decode step makes a hundred of these calls, and one of
+# them costs the device a few microseconds only.
+_E4M3, _F32, _BF16 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
+_BOTH = {_F32: DTYPE_CODES[_F32], _BF16: DTYPE_CODES[_BF16]}
+_ONLY_F32 = {_F32: DTYPE_CODES[_F32]}
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _device_index(ctx: StepContext) -> int:
+    device = ctx.device
+    if device.index is not None:
+        return device.index
+    return -1 if device.type == "cpu" else _current_device()
+
+
+def _rows(name: str, m: Float8Rows, index: int) -> tuple[int, int, int, int, int]:
+    """Checks rows in 8 bits; their address and pitch, the scales' address, rows and columns."""
     v, s = m.values, m.scales
-    if (v.dtype == torch.float8_e4m3fn and v.dim() == 2 and (v.stride(1) == 1 or v.shape[1] <= 1) and v.device == device and v.data_ptr() % ROW_BYTES == 0
-            and (v.shape[0] <= 1 or (v.stride(0) % ROW_BYTES == 0 and v.stride(0) >= v.shape[1]))
-            and s.dtype == torch.float32 and s.shape == v.shape[:1] and s.is_contiguous() and s.device == device):
-        return
-    _need(False, f"float8: {name} must be e4m3 [rows, columns] whose rows are contiguous on 16-byte boundaries, with float32 [rows] scales, on {device}; "
-                 f"got {v.dtype} {list(v.shape)} (strides {list(v.stride())}, {v.device}) and {s.dtype} {list(s.shape)} ({s.device})")
+    shape = v.shape
+    if len(shape) == 2:
+        rows, columns = shape
+        pitch, step = v.stride()
+        if rows <= 1 or columns == 0:
+            pitch = -(-columns // ROW_BYTES) * ROW_BYTES
+        address = v.data_ptr()
+        if (v.dtype is _E4M3 and (step == 1 or columns <= 1) and not (address | pitch) % ROW_BYTES and pitch >= columns and v.get_device() == index
+                and s.dtype is _F32 and s.shape == (rows,) and (rows <= 1 or s.stride(0) == 1) and s.get_device() == index and rows < 2**31 and columns < 2**31):
+            return address, pitch, s.data_ptr(), rows, columns
+    raise KernelError(f"float8: {name} must be e4m3 [rows, columns] whose rows are contiguous on 16-byte boundaries, with float32 [rows] scales, on "
+                      f"{_device_name(index)}; got {v.dtype} {list(v.shape)} (strides {list(v.stride())}, {v.device}) and {s.dtype} {list(s.shape)} ({s.device})")
 
 
-def _need_matrix(name: str, t: torch.Tensor, shape: tuple[int, int], dtypes: tuple[torch.dtype, ...], device: torch.device) -> int:
-    """Checks a matrix with contiguous rows, some distance apart; returns that distance."""
-    if t.dtype not in dtypes or tuple(t.shape) != shape or t.device != device or (t.stride(1) != 1 and shape[1] > 1) or (shape[0] > 1 and t.stride(0) < shape[1]):
-        _need(False, f"float8: {name} must be {' or '.join(str(d).removeprefix('torch.') for d in dtypes)} {list(shape)} with contiguous rows on {device}; "
-                     f"got {t.dtype} {list(t.shape)} (strides {list(t.stride())}, {t.device})")
-    return t.stride(0) if shape[0] > 1 else -(-shape[1] // 8) * 8
+def _matrix(name: str, t: torch.Tensor, rows: int, columns: int, dtypes: dict[torch.dtype, int], index: int) -> tuple[int, int, int]:
+    """Checks a matrix whose rows are contiguous, some distance apart; its address, that distance and its type's code."""
+    code = dtypes.get(t.dtype)
+    if code is not None and t.shape == (rows, columns) and t.get_device() == index:
+        pitch, step = t.stride()
+        if rows <= 1:
+            pitch = -(-columns // 8) * 8
+        if (step == 1 or columns <= 1) and pitch >= columns:
+            return t.data_ptr(), pitch, code
+    raise KernelError(f"float8: {name} must be {' or '.join(str(d).removeprefix('torch.') for d in dtypes)} {[rows, columns]} with contiguous rows on "
+                      f"{_device_name(index)}; got {t.dtype} {list(t.shape)} (strides {list(t.stride())}, {t.device})")
 
 
-_BOTH = (torch.float32, torch.bfloat16)
-_F32 = (torch.float32,)
+def _vector(name: str, t: torch.Tensor, count: int, index: int) -> int:
+    if t.dtype is _F32 and t.shape == (count,) and (count <= 1 or t.stride(0) == 1) and t.get_device() == index:
+        return t.data_ptr()
+    raise KernelError(f"float8: {name} must be float32 [{count}] on {_device_name(index)}; got {t.dtype} {list(t.shape)} ({t.device})")
 
 
-def _call(ctx: StepContext, name: str, *args) -> None:
+def _device_name(index: int) -> str:
+    return "cpu" if index < 0 else f"cuda:{index}"
+
+
+# A call's numbers travel as one block (the structs of the same names in csrc/kernels): one argument each took 4 us a product.
+_pack_quantize = Struct("8q").pack
+_pack_rmsnorm = Struct("13qd").pack
+_pack_linear = Struct("19q").pack
+
+
+def _call(ctx: StepContext, index: int, name: str, block: bytes) -> None:
     """Launches on the step's device, whichever is current."""
-    if torch.cuda.current_device() == ctx.device.index or ctx.device.index is None:
-        ctx.lib.call(name, *args, ctx.stream)
+    if _current_device() == index:
+        ctx.lib.call(name, block, ctx.stream)
     else:
-        with torch.cuda.device(ctx.device):
-            ctx.lib.call(name, *args, ctx.stream)
-
-
-def _need_size(*sizes: int) -> None:
-    _need(all(s < 2**31 for s in sizes), "float8: rows and columns are counted in 31 bits")
+        with torch.cuda.device(index):
+            ctx.lib.call(name, block, ctx.stream)
 
 
 def quantize(ctx: StepContext, x: torch.Tensor, out: Float8Rows) -> Float8Rows:
     """``out`` = the rows of ``x`` (float32 or bfloat16, rows contiguous) in 8 bits: ``scale = max(max |row| / 448, 2**-126)``, numbers over it
     rounded to the nearest (ties to even). NaN stays in its place; a row with an infinity has scale infinity, zeros and NaN."""
-    rows, columns = out.shape
-    _need(columns > 0, "float8: rows without numbers have no scale")
-    _need_rows("out", out, x.device)
-    stride = _need_matrix("x", x, out.shape, _BOTH, ctx.device)
-    _need_size(rows, columns)
-    _call(ctx, "b200_float8_quantize", ptr(x), c_int(DTYPE_CODES[x.dtype]), c_int64(stride), ptr(out.values), c_int64(out.row_stride), ptr(out.scales),
-          c_int(rows), c_int(columns))
+    index = _device_index(ctx)
+    o, o_pitch, scales, rows, columns = _rows("out", out, index)
+    if columns == 0:
+        raise KernelError("float8: rows without numbers have no scale")
+    x_at, x_pitch, code = _matrix("x", x, rows, columns, _BOTH, index)
+    _call(ctx, index, "b200_float8_quantize", _pack_quantize(x_at, code, x_pitch, o, o_pitch, scales, rows, columns))
     return out
 
 
@@ -136,38 +164,39 @@ def rmsnorm(ctx: StepContext, x: torch.Tensor, delta: torch.Tensor | None, weigh
             stream: torch.Tensor | None = None) -> Float8Rows:
     """``s = x + delta`` and ``out`` = the rows ``s * rsqrt(mean(s^2) + eps) * weight`` in 8 bits (:func:`quantize`). ``x`` is the 32-bit residual stream;
     the sum goes to ``stream``, by default back into ``x`` (with no ``delta`` nothing is written unless ``stream`` is given)."""
-    rows, columns = out.shape
-    _need(columns > 0, "float8: rows without numbers have no scale")
-    _need_rows("out", out, x.device)
-    x_stride = _need_matrix("x", x, out.shape, _F32, ctx.device)
-    delta_stride = _need_matrix("delta", delta, out.shape, _BOTH, ctx.device) if delta is not None else 0
-    if stream is None and delta is not None:
-        stream = x
-    stream_stride = _need_matrix("stream", stream, out.shape, _F32, ctx.device) if stream is not None else 0
-    _need(weight.dtype == torch.float32 and weight.shape == (columns,) and weight.is_contiguous() and weight.device == ctx.device,
-          "float8: the norm's weight must be float32 [columns]")
-    _need_size(rows, columns)
-    _call(ctx, "b200_float8_rmsnorm", ptr(x), c_int64(x_stride), ptr(delta), c_int(DTYPE_CODES[delta.dtype] if delta is not None else 0), c_int64(delta_stride),
-          ptr(weight), c_float(eps), ptr(stream), c_int64(stream_stride), ptr(out.values), c_int64(out.row_stride), ptr(out.scales), c_int(rows), c_int(columns))
+    index = _device_index(ctx)
+    o, o_pitch, scales, rows, columns = _rows("out", out, index)
+    if columns == 0:
+        raise KernelError("float8: rows without numbers have no scale")
+    x_at, x_pitch, _ = _matrix("x", x, rows, columns, _ONLY_F32, index)
+    d_at, d_pitch, code = (0, 0, 0) if delta is None else _matrix("delta", delta, rows, columns, _BOTH, index)
+    if stream is not None:
+        s_at, s_pitch, _ = _matrix("stream", stream, rows, columns, _ONLY_F32, index)
+    else:
+        s_at, s_pitch = (0, 0) if delta is None else (x_at, x_pitch)
+    _call(ctx, index, "b200_float8_rmsnorm", _pack_rmsnorm(x_at, x_pitch, d_at, code, d_pitch, _vector("the norm's weight", weight, columns, index), s_at, s_pitch,
+                                                           o, o_pitch, scales, rows, columns, eps))
     return out
 
 
-def _product(ctx: StepContext, x: Float8Rows, weight: Float8Rows, out: torch.Tensor, width: int, bias, residual, kind: int, activation: str | None) -> torch.Tensor:
-    _need_rows("x", x, ctx.device)
-    _need_rows("weight", weight, ctx.device)
-    (m, k), (n, inner) = x.shape, weight.shape
-    _need(k == inner and k > 0, f"float8: x is {[m, k]} but weight is {[n, inner]}")
-    _need_size(m, n, k)
-    out_stride = _need_matrix("out", out, (m, width), _BOTH, ctx.device)
-    _need(bias is None or (bias.dtype == torch.float32 and bias.shape == (n,) and bias.is_contiguous() and bias.device == ctx.device),
-          f"float8: bias must be float32 [{n}]")
-    residual_stride = _need_matrix("residual", residual, (m, n), _F32, ctx.device) if residual is not None else 0
-    if m == 0 or n == 0:
-        return out
-    _call(ctx, "b200_float8_linear", ptr(x.values), c_int64(x.row_stride), ptr(x.scales), ptr(weight.values), c_int64(weight.row_stride), ptr(weight.scales),
-          c_int(int(weight.constant)), ptr(out), c_int(DTYPE_CODES[out.dtype]), c_int64(out_stride), ptr(bias), ptr(residual), c_int64(residual_stride),
-          c_int(m), c_int(n), c_int(k), c_int(kind), c_int(ACTIVATIONS[activation]), ptr(ctx.err))
+def _product(ctx: StepContext, x: Float8Rows, weight: Float8Rows, out: torch.Tensor, bias, residual, kind: int, activation: int) -> torch.Tensor:
+    index = _device_index(ctx)
+    x_at, x_pitch, x_scales, m, k = _rows("x", x, index)
+    w_at, w_pitch, w_scales, n, inner = _rows("weight", weight, index)
+    if k != inner or k == 0:
+        raise KernelError(f"float8: x is {[m, k]} but weight is {[n, inner]}")
+    if kind == _GATED and n % 2:
+        raise KernelError(f"float8: gate and up rows come in pairs, weight has {n} rows")
+    o, o_pitch, code = _matrix("out", out, m, n // 2 if kind == _GATED else n, _BOTH, index)
+    b = 0 if bias is None else _vector("bias", bias, n, index)
+    r, r_pitch, _ = (0, 0, 0) if residual is None else _matrix("residual", residual, m, n, _ONLY_F32, index)
+    if m and n:
+        _call(ctx, index, "b200_float8_linear", _pack_linear(x_at, x_pitch, x_scales, w_at, w_pitch, w_scales, weight.constant, o, code, o_pitch, b, r, r_pitch,
+                                                             m, n, k, kind, activation, ctx.err.data_ptr()))
     return out
+
+
+_PLAIN, _ACTIVATED, _GATED = 0, 1, 2
 
 
 def linear(ctx: StepContext, x: Float8Rows, weight: Float8Rows, out: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
@@ -175,14 +204,15 @@ def linear(ctx: StepContext, x: Float8Rows, weight: Float8Rows, out: torch.Tenso
     """``out = act(x @ weight.T + bias) + residual`` in one kernel; ``weight`` is ``[out_features, in_features]``, ``out`` bfloat16 or float32 with
     contiguous rows, ``bias`` float32, ``activation`` None, ``"silu"``, ``"gelu"`` (tanh form) or ``"squared_relu"``, ``residual`` float32 (it may be
     ``out`` itself). Sums are 32-bit and rounded once on the way out."""
-    _need(activation in ACTIVATIONS, f"float8: no activation {activation!r} (there are {', '.join(str(a) for a in ACTIVATIONS)})")
-    return _product(ctx, x, weight, out, weight.shape[0], bias, residual, 0 if activation is None else 1, activation)
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise KernelError(f"float8: no activation {activation!r} (there are {', '.join(str(a) for a in ACTIVATIONS)})")
+    return _product(ctx, x, weight, out, bias, residual, _ACTIVATED if code else _PLAIN, code)
 
 
 def linear_gated(ctx: StepContext, x: Float8Rows, weight: Float8Rows, out: torch.Tensor, activation: str = "silu", bias: torch.Tensor | None = None) -> torch.Tensor:
     """``out = act(gate) * up`` of ``x @ weight.T + bias`` with interleaved gate/up rows (row 2j is gate_j, row 2j + 1 up_j): both projections, the
     activation (``"silu"`` or ``"gelu"``) and the product in one kernel."""
-    _need(activation in GATED_ACTIVATIONS, f"float8: no gated activation {activation!r} (there are {', '.join(GATED_ACTIVATIONS)})")
-    n = weight.shape[0]
-    _need(n % 2 == 0, f"float8: gate and up rows come in pairs, weight has {n} rows")
-    return _product(ctx, x, weight, out, n // 2, bias, None, 2, activation)
+    if activation not in GATED_ACTIVATIONS:
+        raise KernelError(f"float8: no gated activation {activation!r} (there are {', '.join(GATED_ACTIVATIONS)})")
+    return _product(ctx, x, weight, out, bias, None, _GATED, ACTIVATIONS[activation])

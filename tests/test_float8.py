@@ -50,7 +50,7 @@ def test_from_tensor_is_the_nearest(dtype, shape):
     torch.manual_seed(3)
     w = (torch.randn(shape) * 0.02).to(dtype)
     rows = float8.from_tensor(w)
-    assert rows.constant and rows.shape == shape and rows.values.data_ptr() % 16 == 0 and (shape[0] == 1 or rows.row_stride % 16 == 0)
+    assert rows.constant and rows.shape == shape and rows.values.data_ptr() % 16 == 0 and (shape[0] == 1 or rows.values.stride(0) % 16 == 0)
     check_rows(rows, w.double(), 2.0**-23, 2.0**-22)
     torch.testing.assert_close(rows.dequantized().double(), w.double(), rtol=2.0**-4 + 2.0**-20, atol=float(w.abs().max()) * 2.0**-9 / 448)
 
