@@ -114,7 +114,8 @@ constexpr int kStageFloats = 8 * 32;
 template <int KIND, typename T>
 class WayOut {
  public:
-  __device__ __forceinline__ WayOut(const Epilogue& e, int m0, int n0, float* stage) : e_(e), stage_(stage) {
+  // apart: tokens from one eight to the next.
+  __device__ __forceinline__ WayOut(const Epilogue& e, int m0, int n0, float* stage, int apart = 8) : e_(e), stage_(stage), apart_(apart) {
     const int lane = threadIdx.x & 31;
     ws_ = b_ = 0.f;
     if (n0 + lane < e.N) {
@@ -143,7 +144,7 @@ class WayOut {
 #pragma unroll
         for (int q = 0; q < 2; ++q) r[q] = q * 4 + (lane >> 3) < left ? residual_quad(e_, m_ + q * 4 + (lane >> 3), n_) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      from_ += 8 * e_.residual_stride;
+      from_ += apart_ * e_.residual_stride;
     }
     const float2 ws = make_float2(ws_, ws_), b = make_float2(b_, b_);
 #pragma unroll
@@ -179,14 +180,15 @@ class WayOut {
       for (int q = 0; q < 2; ++q)
         if (q * 4 + (lane >> 3) < left) store_some<KIND, T>(to_ + q * 4 * e_.out_stride, n_, e_.N, q == 0 ? mine[0] : mine[1], e_.activation);
     }
-    to_ += 8 * e_.out_stride;
-    m_ += 8;
+    to_ += apart_ * e_.out_stride;
+    m_ += apart_;
     __syncwarp();
   }
 
  private:
   const Epilogue& e_;
   float* stage_;
+  int apart_;
   float ws_, b_;
   int m_, n_;
   bool whole_;
@@ -296,6 +298,8 @@ struct Product {
   int* err;
 };
 
+// csrc/kernels/gemm_float8_skinny.cu: up to 16 tokens and a short stream of weights.
+int launch_skinny(const Product& p, cudaStream_t stream);
 // csrc/kernels/gemm_float8_stream.cu: weights streamed past few tokens, K split inside clusters.
 int launch_stream(const Product& p, cudaStream_t stream);
 // csrc/kernels/gemm_float8_tiles.cu: pairs of SMs on tiles of 256 rows of W by up to 256 tokens.

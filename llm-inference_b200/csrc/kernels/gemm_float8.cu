@@ -78,6 +78,7 @@ B200_API int b200_float8_linear(const Float8Linear* c, cudaStream_t stream) {
   const int size = p.out_f32 ? 4 : 2, at_once = p.kind == GATED ? 2 : 4;  // outputs from four rows of W
   e.vector = e.out_stride % at_once == 0 && reinterpret_cast<uintptr_t>(e.out) % (at_once * size) == 0 &&
              (e.residual == nullptr || (e.residual_stride % 4 == 0 && reinterpret_cast<uintptr_t>(e.residual) % 16 == 0));
+  if (float8::g_tile == -1) return launch_skinny(p, stream);
   if (float8::g_tile > 0) return launch_tiles(p, float8::g_tile, stream);
   return launch_stream(p, stream);
 }

@@ -3,11 +3,12 @@
 //
 // W is the wide operand: a block owns 128 rows of W (the MMA's M) and a tile of up to 128 tokens (its N, a multiple of 16). One thread fills a ring
 // of stages by TMA (128 rows x 128 bytes of W, tokens x 128 bytes of X, 128-byte swizzle), one issues `tcgen05.mma` (kind::f8f6f4, 32 k an
-// instruction) into TMEM, four warps read the sums back, a lane per row of W. Where W has too few rows to give every SM work, the blocks of a
-// cluster share rows and split K: each sends its partial sums to the shared memory of the member that finishes those rows, and the owners add in
-// member order, so a sum does not depend on timing. With up to 16 tokens the inboxes lie behind the ring, the sums are stored there from registers
-// and the cluster meets once. With more tokens outbox and inbox take the ring's place, so the cluster meets first; a slice then travels as
-// one bulk copy to its owner, who waits for the bytes (64 tokens of 4,608 x 3,584: single stores 9.9 us, copies TIME_BULK).
+// instruction) into TMEM, eight warps read the sums back, a lane per row of W. Where W has too few rows to give every SM work, the blocks of a
+// cluster share rows and split K: each sends its partial sums to the members that finish those rows, a slice each, and the owners add in member
+// order, so a sum does not depend on timing. A block puts its sums where its ring was, one bulk copy per owner takes them to an inbox behind the
+// owner's ring, and the owner waits for the bytes: nobody waits for a member that has nothing to do with its rows, and the cluster meets only to
+// know that barriers are there and, on leaving, that copies have been read. (64 tokens of 4,608 x 3,584: 11.1 us with the cluster meeting
+// three times and single stores into neighbours' memory, TIME_BULK so.)
 //
 // 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as TMEM goes, added up as they are read.
 //
@@ -23,10 +24,10 @@
 namespace float8 {
 namespace {
 
-constexpr int kThreads = 192;      // warp 0: TMA, warp 1: MMA, warps 2-5: sums
+constexpr int kSumWarps = 8;       // two a quarter of the TMEM lanes
+constexpr int kThreads = (2 + kSumWarps) * 32;  // warp 0: TMA, warp 1: MMA, warps 2-9: sums
 constexpr int kMaxStages = 12;
 constexpr int kMaxMembers = 16;
-constexpr int kEarlyTokens = 16;   // up to this many (padded) tokens the inboxes lie behind the ring
 constexpr int kMaxTokens = 128;    // a block's
 
 struct StreamParams {
@@ -38,6 +39,7 @@ struct StreamParams {
   int chain_blocks;  // k-blocks per accumulator
   int tmem_cols;
   int w_constant;
+  int inbox_at;      // bytes from the ring's start
 };
 
 // Rows of a block that one member of a cluster finishes: whole 32-byte pieces of 32-bit output rows (the last members may have none).
@@ -56,11 +58,6 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
-// Bytes of the outbox: a slice per owner, of the padded tokens.
-__host__ __device__ constexpr size_t outbox_bytes(int members, int tile) {
-  const int slice = slice_rows(members), owners = (kRowsW + slice - 1) / slice;
-  return static_cast<size_t>(owners) * slice * tile * sizeof(float);
-}
 // `bytes` (a multiple of 16) from here to the same place of block `rank`, counted on that block's barrier.
 __device__ __forceinline__ void copy_to_peer(float* dst, const float* src, uint32_t bytes, uint64_t* bar, int rank) {
   asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(peer_address(dst, rank)), "r"(smem_addr(src)),
@@ -68,50 +65,49 @@ __device__ __forceinline__ void copy_to_peer(float* dst, const float* src, uint3
                : "memory");
 }
 
-// What one member finishes: `rows` rows of W from n0 on, the members' partial sums ([members][tokens][slice]) added in member order. An item is four
-// neighbouring rows of one token; a thread takes kItems of them at a time and asks for everything from memory before it adds.
+// What one member finishes: `rows` rows of W from n0 on, the members' partial sums ([members][tokens][slice]) added in member order; `scales` and
+// `bias` are those rows'. An item is four neighbouring rows of one token; a thread takes kItems of them at a time.
 template <int KIND, typename T>
-__device__ __forceinline__ void finish_slice(const Epilogue& e, const float* inbox, const float* x_scales, int m0, int tokens, int n0, int rows, int slice, int members) {
+__device__ __forceinline__ void finish_slice(const Epilogue& e, const float* inbox, const float* x_scales, const float* scales, const float* bias, int m0, int tokens,
+                                             int n0, int rows, int slice, int members) {
   constexpr int kItems = 2;
   const int quads = (min(rows, e.N - n0) + 3) / 4;  // with rows of W left
   const int total = quads * tokens, plane = tokens * slice;
   for (int base = threadIdx.x; base < total; base += kThreads * kItems) {
     int m[kItems], j[kItems];
-    float4 sum[kItems], ws[kItems], b[kItems], r[kItems];
+    float4 sum[kItems], r[kItems];
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
       const int item = min(base + u * kThreads, total - 1);
       m[u] = item / quads;
       j[u] = 4 * (item - m[u] * quads);
-      const int n = n0 + j[u], last = e.N - 1;
-      ws[u] = make_float4(e.w_scale[n], e.w_scale[min(n + 1, last)], e.w_scale[min(n + 2, last)], e.w_scale[min(n + 3, last)]);
-      b[u] = r[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (e.bias != nullptr) b[u] = make_float4(e.bias[n], e.bias[min(n + 1, last)], e.bias[min(n + 2, last)], e.bias[min(n + 3, last)]);
-      if (KIND != GATED && e.residual != nullptr && base + u * kThreads < total) r[u] = residual_quad(e, m0 + m[u], n);
+      r[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (KIND != GATED && e.residual != nullptr && base + u * kThreads < total) r[u] = residual_quad(e, m0 + m[u], n0 + j[u]);
       sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     for (int member = 0; member < members; ++member) {
 #pragma unroll
-      for (int u = 0; u < kItems; ++u) {
-        const float4 part = *reinterpret_cast<const float4*>(inbox + member * plane + m[u] * slice + j[u]);
-        sum[u] = make_float4(sum[u].x + part.x, sum[u].y + part.y, sum[u].z + part.z, sum[u].w + part.w);
-      }
+      for (int u = 0; u < kItems; ++u) sum[u] = add_each(sum[u], *reinterpret_cast<const float4*>(inbox + member * plane + m[u] * slice + j[u]));
     }
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
       if (base + u * kThreads >= total) break;
-      const float xs = x_scales[m[u]];
-      float4 v = make_float4(fmaf(sum[u].x * xs, ws[u].x, b[u].x), fmaf(sum[u].y * xs, ws[u].y, b[u].y), fmaf(sum[u].z * xs, ws[u].z, b[u].z),
-                                   fmaf(sum[u].w * xs, ws[u].w, b[u].w));
-      const int n = n0 + j[u];
+      const float4 ws = *reinterpret_cast<const float4*>(scales + j[u]), b = *reinterpret_cast<const float4*>(bias + j[u]);
+      float4 v = fma_each(scale_each(sum[u], x_scales[m[u]]), ws, b);
       if constexpr (KIND == ACTIVATED) v = activate_quad(v, e.activation);
       if constexpr (KIND != GATED) v = add_each(v, r[u]);
+      const int n = n0 + j[u];
       T* to = static_cast<T*>(e.out) + (m0 + m[u]) * e.out_stride + (KIND == GATED ? n >> 1 : n);
       if (e.vector && n + 3 < e.N) store_whole<KIND, T>(to, v, e.activation);
       else store_some<KIND, T>(to, n, e.N, v, e.activation);
     }
   }
 }
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+// Without waiting for this thread's stores to be seen: what it says is that copies have come.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // A form carries no code that it does not take: a block runs its epilogue once, from a cold instruction cache (measured in gemm_tcgen05.cu).
 template <int KIND, typename T, bool CLUSTERED>
@@ -128,7 +124,8 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   __shared__ __align__(8) uint64_t inbox_bar;
   __shared__ uint32_t tmem_base_shared;
   __shared__ __align__(16) float x_scales[kMaxTokens];
-  __shared__ __align__(16) float stages_out[CLUSTERED ? 4 : 4 * kStageFloats];
+  // Clustered: the scales and bias of the rows that this member finishes. Otherwise the warps' way out of TMEM.
+  __shared__ __align__(16) float rows_out[CLUSTERED ? 2 * kRowsW : kSumWarps * kStageFloats];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int stages = p.stages;
@@ -160,7 +157,13 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     wait_for_predecessor();
     for (int i = 0; i < first; ++i) load_x(i);
   }
+  if constexpr (CLUSTERED) {
+    __syncwarp();
+    cluster_arrive();  // this block's barriers are there
+  }
   wait_for_predecessor();
+  const int slice = CLUSTERED ? slice_rows(members) : 0;
+  const int mine = rank * slice, rows = max(0, min(kRowsW - mine, slice));  // the rows this member finishes, from n0 + mine on
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_shared)),
                  "r"(static_cast<uint32_t>(p.tmem_cols))
@@ -168,7 +171,18 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (warp >= 2) {
-    for (int i = threadIdx.x - 64; i < p.tile; i += 128) x_scales[i] = m0 + i < p.e.M ? p.e.x_scale[m0 + i] : 0.f;
+    const int tid = threadIdx.x - 64;
+    if (tid < p.tile) x_scales[tid] = m0 + tid < p.e.M ? p.e.x_scale[m0 + tid] : 0.f;
+    if constexpr (CLUSTERED) {
+      if (tid < rows) {
+        const int n = n0 + mine + tid;
+        rows_out[tid] = n < p.e.N ? p.e.w_scale[n] : 0.f;
+        rows_out[kRowsW + tid] = p.e.bias != nullptr && n < p.e.N ? p.e.bias[n] : 0.f;
+      }
+      // The residual will be wanted all at once.
+      if (KIND != GATED && p.e.residual != nullptr && m0 + tid < p.e.M && tid < p.tile && n0 + mine < p.e.N)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.e.residual + (m0 + tid) * p.e.residual_stride + n0 + mine));
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -220,65 +234,53 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   __syncwarp();
 
   const int tokens = min(p.tile, p.e.M - m0);
-  const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31 belong to this warp
-  const int row = quarter * 32 + lane;
-  if (warp >= 2) {
-    const bool have = mbar_wait(&accum_bar, 0);
-    if (!have && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if constexpr (!CLUSTERED) {
-      const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
-      WayOut<KIND, T> way(p.e, m0, n0 + quarter * 32, stages_out + (warp - 2) * kStageFloats);
-      for (int c0 = 0; have && c0 < tokens; c0 += 8) {
+  const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
+  const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31 belong to this warp, every other eight tokens too
+  const int side = (warp - 2) >> 2;
+  const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+  if constexpr (!CLUSTERED) {
+    if (warp >= 2) {
+      WayOut<KIND, T> way(p.e, m0 + side * 8, n0 + quarter * 32, rows_out + (warp - 2) * kStageFloats, 16);
+      const bool have = mbar_wait(&accum_bar, 0);
+      if (!have && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      for (int c0 = side * 8; have && c0 < tokens; c0 += 16) {
         float v[8];
-        tmem_sums(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, chains, p.tile, v);
+        tmem_sums(lanes + c0, chains, p.tile, v);
         way.take(x_scales + c0, v);
       }
     }
-  }
-  if constexpr (CLUSTERED) {
-    const int slice = slice_rows(members);
-    const int chains = (num_kb + p.chain_blocks - 1) / p.chain_blocks;
-    const bool early = p.tile <= kEarlyTokens;
-    const int plane = tokens * slice;  // what one member sends to one owner: [tokens][slice]
-    const int owner = row / slice, in_slice = row - owner * slice;
-    const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    float* inbox = reinterpret_cast<float*>(tiles + (early ? static_cast<size_t>(stages) * stage_bytes : outbox_bytes(members, p.tile)));  // [members][plane]
-    if (early) {
-      if (warp >= 2) {
-        const uint32_t mine = peer_address(inbox + rank * plane + in_slice, owner);
-        for (int c0 = 0; c0 < tokens; c0 += 8) {
-          float v[8];
-          tmem_sums(lanes + c0, chains, p.tile, v);
+  } else {
+    cluster_wait();  // the other members' barriers are there
+    float* outbox = reinterpret_cast<float*>(tiles);  // [owners][tokens][slice], where the ring was
+    float* inbox = reinterpret_cast<float*>(tiles + p.inbox_at);  // [members][tokens][slice]
+    const int plane = tokens * slice;
+    if (warp >= 2) {
+      if (!mbar_wait(&accum_bar, 0) && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int row = quarter * 32 + lane, owner = row / slice;
+      float* to = outbox + owner * plane + (row - owner * slice);
+      for (int c0 = side * 8; c0 < tokens; c0 += 16) {
+        float v[8];
+        tmem_sums(lanes + c0, chains, p.tile, v);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c0 + i < tokens) store_peer_f32(mine + static_cast<uint32_t>((c0 + i) * slice) * sizeof(float), v[i]);
-        }
+        for (int i = 0; i < 8; ++i)
+          if (c0 + i < tokens) to[(c0 + i) * slice] = v[i];
       }
-      cluster_sync_all();
-    } else {
-      float* outbox = reinterpret_cast<float*>(tiles);  // [owners][plane]
-      cluster_sync_all();  // nobody's ring is read any more
-      if (warp >= 2) {
-        float* mine = outbox + owner * plane + in_slice;
-        for (int c0 = 0; c0 < tokens; c0 += 8) {
-          float v[8];
-          tmem_sums(lanes + c0, chains, p.tile, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c0 + i < tokens) mine[(c0 + i) * slice] = v[i];
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const uint32_t bytes = static_cast<uint32_t>(plane) * sizeof(float);
-        if (threadIdx.x == 64 && rank * slice < kRowsW) mbar_expect_tx(&inbox_bar, members * bytes);
-        const int to = threadIdx.x - 64;  // a thread per owner
-        if (to < members && to * slice < kRowsW) copy_to_peer(inbox + rank * plane, outbox + to * plane, bytes, &inbox_bar, to);
-      }
-      if (rank * slice < kRowsW && !mbar_wait(&inbox_bar, 0) && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const uint32_t bytes = static_cast<uint32_t>(plane) * sizeof(float);
+      if (threadIdx.x == 64 && rows > 0) mbar_expect_tx(&inbox_bar, members * bytes);
+      const int peer = threadIdx.x - 64;  // a thread per owner
+      if (peer < members && peer * slice < kRowsW) copy_to_peer(inbox + rank * plane, outbox + peer * plane, bytes, &inbox_bar, peer);
     }
-    finish_slice<KIND, T>(p.e, inbox, x_scales, m0, tokens, n0 + rank * slice, max(0, min(kRowsW - rank * slice, slice)), slice, members);
-    if (!early) cluster_sync_all();  // nobody's outbox is read any more
+    __syncwarp();
+    if (rows > 0 && !mbar_wait(&inbox_bar, 0) && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
+    __syncwarp();
+    cluster_arrive_relaxed();  // what was sent here has come
+    finish_slice<KIND, T>(p.e, inbox, x_scales, rows_out, rows_out + kRowsW, m0, tokens, n0 + mine, rows, slice, members);
+    __syncwarp();
+    cluster_wait();  // what was sent from here has been read
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -324,6 +326,7 @@ bool prepare_kernel(StreamKernel kernel) {
 struct StreamPlan {
   int blocks, members, tiles, tile, stages, chain_blocks, tmem_cols;
   size_t smem;
+  int inbox_at;
 };
 
 // How many clusters of `members` blocks run at once with one block an SM (clusters do not straddle GPCs); 0 if it cannot be told.
@@ -365,13 +368,19 @@ void size_ring(StreamPlan& plan, int k_blocks, bool f32) {
   while (plan.tmem_cols < accumulators * plan.tile) plan.tmem_cols *= 2;
   size_t budget = alone ? 190 * 1024 : (plan.blocks * plan.members * plan.tiles <= 2 * b200_sm_count_host() ? 100 * 1024 : 66 * 1024);
   if (g_override.budget > 0) budget = static_cast<size_t>(g_override.budget) * 1024;
+  if (plan.members > 1) budget -= min(budget / 2, static_cast<size_t>(plan.members) * slice_rows(plan.members) * plan.tile * sizeof(float));  // the inbox
   int stages = static_cast<int>(budget / stage);
   if (g_override.stages > 0) stages = g_override.stages;
   stages = min(min(stages, kMaxStages), per_block);
   plan.stages = max(stages, 2);
-  const size_t ring = plan.stages * stage;
-  const size_t inbox = plan.members > 1 ? static_cast<size_t>(plan.members) * slice_rows(plan.members) * plan.tile * sizeof(float) : 0;
-  plan.smem = (plan.tile <= kEarlyTokens ? ring + inbox : max(ring, inbox > 0 ? outbox_bytes(plan.members, plan.tile) + inbox : 0)) + 1024;
+  size_t ring = plan.stages * stage, inbox = 0;
+  if (plan.members > 1) {
+    const int slice = slice_rows(plan.members), owners = (kRowsW + slice - 1) / slice;
+    ring = max(ring, static_cast<size_t>(owners) * slice * plan.tile * sizeof(float));  // the outbox takes its place
+    inbox = static_cast<size_t>(plan.members) * slice * plan.tile * sizeof(float);
+  }
+  plan.inbox_at = static_cast<int>(ring);
+  plan.smem = ring + inbox + 1024;
   if (alone) plan.smem = max(plan.smem, static_cast<size_t>(118 * 1024));  // TMEM goes with shared memory: see the head of the file
   else plan.smem = max(plan.smem, static_cast<size_t>(plan.tmem_cols) * 227 * 1024 / 512);
 }
@@ -442,6 +451,7 @@ int launch_stream(const Product& product, cudaStream_t stream) {
   p.chain_blocks = plan.chain_blocks;
   p.tmem_cols = plan.tmem_cols;
   p.w_constant = product.w_constant;
+  p.inbox_at = plan.inbox_at;
   CUtensorMap w_map, x_map;
   if (make_map(&w_map, product.w, e.N, product.K, product.w_stride, kRowsW) != 0) return -1;
   if (make_map(&x_map, product.x, e.M, product.K, product.x_stride, plan.tile) != 0) return -1;
