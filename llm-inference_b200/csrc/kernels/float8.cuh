@@ -268,7 +268,7 @@ __device__ __forceinline__ void tmem_store(uint32_t taddr, const float (&v)[8]) 
                : "memory");
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// The same eight columns of `chains` accumulators, `apart` columns from one to the next, added in order.
+// The same eight columns of `chains` accumulators, `apart` columns from one to the next, added in order; and of two places at once.
 __device__ __forceinline__ void tmem_sums(uint32_t taddr, int chains, int apart, float (&v)[8]) {
   tmem_ask(taddr, v);
   tmem_wait(v);
@@ -278,6 +278,23 @@ __device__ __forceinline__ void tmem_sums(uint32_t taddr, int chains, int apart,
     tmem_wait(more);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += more[i];
+  }
+}
+__device__ __forceinline__ void tmem_sums(uint32_t first, uint32_t second, int chains, int apart, float (&v)[2][8]) {
+  tmem_ask(first, v[0]);
+  tmem_ask(second, v[1]);
+  tmem_wait(v[0]);
+  tmem_wait(v[1]);
+  for (int c = 1; c < chains; ++c) {
+    float more[2][8];
+    tmem_ask(first + c * apart, more[0]);
+    tmem_ask(second + c * apart, more[1]);
+    tmem_wait(more[0]);
+    tmem_wait(more[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[h][i] += more[h][i];
   }
 }
 

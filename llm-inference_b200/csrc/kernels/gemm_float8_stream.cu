@@ -12,10 +12,11 @@
 //
 // 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as TMEM goes, added up as they are read.
 //
-// The first stages' weights are asked for before the kernel in front has ended where the caller says that nothing still writes them; TMEM is
-// taken only after it has (a block that held TMEM while a kernel in front still wanted some could keep both waiting). A block takes no larger a
-// share of an SM's TMEM than of its shared memory, so a resident block never waits for another's. Every wait is bounded: a block that gives
-// up sets the timeout bit, waits for its copies in flight, frees its TMEM and leaves.
+// The first stages' weights are asked for before the kernel in front has ended where the caller says that nothing still writes them. TMEM is
+// taken first thing: an SM starts no second block that takes TMEM before the first has given up the permit to (measured: with the wait for the kernel in
+// front before it, the second block of every SM began 2.7 us late, with it in front 1.1 us). A block takes no larger a share of an SM's TMEM than of its
+// shared memory, so a resident block never waits for another's. Every wait is bounded: a block that gives up sets the timeout bit, waits for its
+// copies in flight, frees its TMEM and leaves.
 #include <mutex>
 #include <vector>
 
@@ -69,20 +70,20 @@ __device__ __forceinline__ void copy_to_peer(float* dst, const float* src, uint3
 // `bias` are those rows'. An item is four neighbouring rows of one token; a thread takes kItems of them at a time.
 template <int KIND, typename T>
 __device__ __forceinline__ void finish_slice(const Epilogue& e, const float* inbox, const float* x_scales, const float* scales, const float* bias, int m0, int tokens,
-                                             int n0, int rows, int slice, int members) {
-  constexpr int kItems = 2;
+                                             int n0, int rows, int slice, int members, int tid) {
+  constexpr int kItems = 2, kFinishThreads = kSumWarps * 32;
   const int quads = (min(rows, e.N - n0) + 3) / 4;  // with rows of W left
   const int total = quads * tokens, plane = tokens * slice;
-  for (int base = threadIdx.x; base < total; base += kThreads * kItems) {
+  for (int base = tid; base < total; base += kFinishThreads * kItems) {
     int m[kItems], j[kItems];
     float4 sum[kItems], r[kItems];
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
-      const int item = min(base + u * kThreads, total - 1);
+      const int item = min(base + u * kFinishThreads, total - 1);
       m[u] = item / quads;
       j[u] = 4 * (item - m[u] * quads);
       r[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (KIND != GATED && e.residual != nullptr && base + u * kThreads < total) r[u] = residual_quad(e, m0 + m[u], n0 + j[u]);
+      if (KIND != GATED && e.residual != nullptr && base + u * kFinishThreads < total) r[u] = residual_quad(e, m0 + m[u], n0 + j[u]);
       sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     for (int member = 0; member < members; ++member) {
@@ -91,7 +92,7 @@ __device__ __forceinline__ void finish_slice(const Epilogue& e, const float* inb
     }
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
-      if (base + u * kThreads >= total) break;
+      if (base + u * kFinishThreads >= total) break;
       const float4 ws = *reinterpret_cast<const float4*>(scales + j[u]), b = *reinterpret_cast<const float4*>(bias + j[u]);
       float4 v = fma_each(scale_each(sum[u], x_scales[m[u]]), ws, b);
       if constexpr (KIND == ACTIVATED) v = activate_quad(v, e.activation);
@@ -117,7 +118,7 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   const uint32_t w_bytes = kRowsW * kBlockK;
   const uint32_t x_bytes = static_cast<uint32_t>(p.tile) * kBlockK;
   const uint32_t stage_bytes = w_bytes + ((x_bytes + 1023u) & ~1023u);
-  unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* tiles = smem_raw + (-smem_addr(smem_raw) & 1023u);
   __shared__ __align__(8) uint64_t full_bar[kMaxStages];
   __shared__ __align__(8) uint64_t empty_bar[kMaxStages];
   __shared__ __align__(8) uint64_t accum_bar;
@@ -140,6 +141,12 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   auto load_w = [&](int i) { tma_load_2d(tiles + (i % stages) * stage_bytes, &w_map, &full_bar[i % stages], (kb_begin + i) * kBlockK, n0); };
   auto load_x = [&](int i) { tma_load_2d(tiles + (i % stages) * stage_bytes + w_bytes, &x_map, &full_bar[i % stages], (kb_begin + i) * kBlockK, m0); };
 
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_shared)),
+                 "r"(static_cast<uint32_t>(p.tmem_cols))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -164,26 +171,6 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   wait_for_predecessor();
   const int slice = CLUSTERED ? slice_rows(members) : 0;
   const int mine = rank * slice, rows = max(0, min(kRowsW - mine, slice));  // the rows this member finishes, from n0 + mine on
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base_shared)),
-                 "r"(static_cast<uint32_t>(p.tmem_cols))
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  if (warp >= 2) {
-    const int tid = threadIdx.x - 64;
-    if (tid < p.tile) x_scales[tid] = m0 + tid < p.e.M ? p.e.x_scale[m0 + tid] : 0.f;
-    if constexpr (CLUSTERED) {
-      if (tid < rows) {
-        const int n = n0 + mine + tid;
-        rows_out[tid] = n < p.e.N ? p.e.w_scale[n] : 0.f;
-        rows_out[kRowsW + tid] = p.e.bias != nullptr && n < p.e.N ? p.e.bias[n] : 0.f;
-      }
-      // The residual will be wanted all at once.
-      if (KIND != GATED && p.e.residual != nullptr && m0 + tid < p.e.M && tid < p.tile && n0 + mine < p.e.N)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.e.residual + (m0 + tid) * p.e.residual_stride + n0 + mine));
-    }
-  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -238,9 +225,12 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31 belong to this warp, every other eight tokens too
   const int side = (warp - 2) >> 2;
   const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+  const int tid = threadIdx.x - 64;  // among the warps that finish
   if constexpr (!CLUSTERED) {
     if (warp >= 2) {
       WayOut<KIND, T> way(p.e, m0 + side * 8, n0 + quarter * 32, rows_out + (warp - 2) * kStageFloats, 16);
+      if (tid < p.tile) x_scales[tid] = m0 + tid < p.e.M ? p.e.x_scale[m0 + tid] : 0.f;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       const bool have = mbar_wait(&accum_bar, 0);
       if (!have && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -256,29 +246,40 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     float* inbox = reinterpret_cast<float*>(tiles + p.inbox_at);  // [members][tokens][slice]
     const int plane = tokens * slice;
     if (warp >= 2) {
+      // While the weights stream: what the finish will want.
+      if (tid < p.tile) x_scales[tid] = tid < tokens ? p.e.x_scale[m0 + tid] : 0.f;
+      if (tid < rows) {
+        const int n = n0 + mine + tid;
+        rows_out[tid] = n < p.e.N ? p.e.w_scale[n] : 0.f;
+        rows_out[kRowsW + tid] = p.e.bias != nullptr && n < p.e.N ? p.e.bias[n] : 0.f;
+      }
+      if (KIND != GATED && p.e.residual != nullptr && tid < tokens && n0 + mine < p.e.N)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.e.residual + (m0 + tid) * p.e.residual_stride + n0 + mine));
       if (!mbar_wait(&accum_bar, 0) && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int row = quarter * 32 + lane, owner = row / slice;
       float* to = outbox + owner * plane + (row - owner * slice);
-      for (int c0 = side * 8; c0 < tokens; c0 += 16) {
-        float v[8];
-        tmem_sums(lanes + c0, chains, p.tile, v);
+      for (int c0 = side * 8; c0 < tokens; c0 += 32) {  // twice eight tokens at a time
+        float v[2][8];
+        const bool second = c0 + 16 < p.tile;
+        tmem_sums(lanes + c0, second ? lanes + c0 + 16 : lanes + c0, chains, p.tile, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c0 + i < tokens) to[(c0 + i) * slice] = v[i];
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c0 + h * 16 + i < tokens) to[(c0 + h * 16 + i) * slice] = v[h][i];
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const uint32_t bytes = static_cast<uint32_t>(plane) * sizeof(float);
-      if (threadIdx.x == 64 && rows > 0) mbar_expect_tx(&inbox_bar, members * bytes);
-      const int peer = threadIdx.x - 64;  // a thread per owner
-      if (peer < members && peer * slice < kRowsW) copy_to_peer(inbox + rank * plane, outbox + peer * plane, bytes, &inbox_bar, peer);
+      if (tid == 0 && rows > 0) mbar_expect_tx(&inbox_bar, members * bytes);
+      if (tid < members && tid * slice < kRowsW) copy_to_peer(inbox + rank * plane, outbox + tid * plane, bytes, &inbox_bar, tid);  // a thread per owner
     }
     __syncwarp();
     if (rows > 0 && !mbar_wait(&inbox_bar, 0) && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
     __syncwarp();
     cluster_arrive_relaxed();  // what was sent here has come
-    finish_slice<KIND, T>(p.e, inbox, x_scales, rows_out, rows_out + kRowsW, m0, tokens, n0 + mine, rows, slice, members);
+    if (warp >= 2) finish_slice<KIND, T>(p.e, inbox, x_scales, rows_out, rows_out + kRowsW, m0, tokens, n0 + mine, rows, slice, members, tid);
     __syncwarp();
     cluster_wait();  // what was sent from here has been read
   }
@@ -382,7 +383,7 @@ void size_ring(StreamPlan& plan, int k_blocks, bool f32) {
   plan.inbox_at = static_cast<int>(ring);
   plan.smem = ring + inbox + 1024;
   if (alone) plan.smem = max(plan.smem, static_cast<size_t>(118 * 1024));  // TMEM goes with shared memory: see the head of the file
-  else plan.smem = max(plan.smem, static_cast<size_t>(plan.tmem_cols) * 227 * 1024 / 512);
+  else plan.smem = max(plan.smem, max(static_cast<size_t>(plan.tmem_cols) * 227 * 1024 / 512, static_cast<size_t>(48 * 1024)));
 }
 
 StreamPlan plan_uncached(int M, int N, int K, bool f32) {

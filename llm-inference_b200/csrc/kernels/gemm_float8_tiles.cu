@@ -11,7 +11,7 @@
 // 32-bit outputs: after each chain of kChainBlocks k-blocks the warps add the sums to registers and the products go on in the other half.
 //
 // Tiles are taken in strips of a few token tiles across all rows of W, so that at any time the clusters share a few rows of both operands in L2.
-// TMEM (all of it) is taken after the kernel in front has ended, shared memory leaves no room for another block. Every wait is bounded: a role that
+// TMEM, all of it, is taken before the kernel in front has ended: shared memory leaves no room for a block of it that still wants some. Every wait is bounded: a role that
 // gives up sets the timeout bit and leaves its loop; copies in flight are waited for, and both blocks meet before either leaves.
 #include "float8.cuh"
 
@@ -82,7 +82,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   const uint32_t w_bytes = kRowsW * kBlockK;
   const uint32_t x_bytes = static_cast<uint32_t>(p.tile / 2) * kBlockK;
   const uint32_t stage_bytes = w_bytes + ((x_bytes + 1023u) & ~1023u);
-  unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* tiles = smem_raw + (-smem_addr(smem_raw) & 1023u);
   __shared__ __align__(8) uint64_t full_bar[kMaxStages];
   __shared__ __align__(8) uint64_t empty_bar[kMaxStages];
   __shared__ __align__(8) uint64_t sums_full[2];
@@ -111,7 +111,6 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  wait_for_predecessor();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_base_shared)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -119,6 +118,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   cluster_sync_all();  // the other block's barriers are there
+  wait_for_predecessor();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   let_successor_start();
   const uint32_t tmem_base = tmem_base_shared;
