@@ -316,10 +316,13 @@ struct Product {
 };
 
 // csrc/kernels/gemm_float8_skinny.cu: up to 16 tokens and a short stream of weights.
+bool skinny_takes(int M, int N, int K);
 int launch_skinny(const Product& p, cudaStream_t stream);
 // csrc/kernels/gemm_float8_stream.cu: weights streamed past few tokens, K split inside clusters.
+float stream_time(const Product& p);
 int launch_stream(const Product& p, cudaStream_t stream);
-// csrc/kernels/gemm_float8_tiles.cu: pairs of SMs on tiles of 256 rows of W by up to 256 tokens.
+// csrc/kernels/gemm_float8_tiles.cu: pairs of SMs on tiles of 256 rows of W by `tile` tokens (64 to 256, a multiple of 32).
+float tiles_time(const Product& p, int tile);
 int launch_tiles(const Product& p, int tile, cudaStream_t stream);
 
 }  // namespace float8

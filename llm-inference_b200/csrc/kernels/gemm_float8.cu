@@ -33,6 +33,21 @@ int make_map(CUtensorMap* map, const void* base, int rows, int K, int64_t stride
   return 0;
 }
 
+// Which kernel. Up to 16 tokens weights are all there is to read: the form for short streams, else the streaming one. With more the faster one by the
+// kernels' own estimates of their time, and the tile form's width with it: tiles fill whole turns of all clusters at different widths (777 tokens
+// of 8,192 x 2,048: 224 tokens 19.9 us, 256 21.3, 160 22.6; 2,048 of 4,608 x 3,584: 256 27.6, 224 33.7).
+static int launch_chosen(const Product& p, cudaStream_t stream) {
+  if (skinny_takes(p.e.M, p.e.N, p.K)) return launch_skinny(p, stream);
+  if (p.e.M <= 16) return launch_stream(p, stream);
+  int best = 0;
+  float least = p.e.M <= 512 ? stream_time(p) : 1e30f;
+  for (int tile = 64; tile <= 256 && (tile == 64 || tile < p.e.M + 32); tile += 32) {
+    const float time = tiles_time(p, tile);
+    if (time < least) least = time, best = tile;
+  }
+  return best == 0 ? launch_stream(p, stream) : launch_tiles(p, best, stream);
+}
+
 }  // namespace float8
 
 // The numbers of a call, in the order in which parts/float8.py packs them: y = epilogue(x w^T), x [M, K] and w [N, K] in e4m3 (pitches in bytes, multiples
@@ -78,8 +93,9 @@ B200_API int b200_float8_linear(const Float8Linear* c, cudaStream_t stream) {
   const int size = p.out_f32 ? 4 : 2, at_once = p.kind == GATED ? 2 : 4;  // outputs from four rows of W
   e.vector = e.out_stride % at_once == 0 && reinterpret_cast<uintptr_t>(e.out) % (at_once * size) == 0 &&
              (e.residual == nullptr || (e.residual_stride % 4 == 0 && reinterpret_cast<uintptr_t>(e.residual) % 16 == 0));
-  if (float8::g_tile == -1) return launch_skinny(p, stream);
-  if (float8::g_tile > 0) return launch_tiles(p, float8::g_tile, stream);
-  return launch_stream(p, stream);
+  if (g_tile == -1) return launch_skinny(p, stream);
+  if (g_tile == -2) return launch_stream(p, stream);
+  if (g_tile > 0) return launch_tiles(p, g_tile, stream);
+  return launch_chosen(p, stream);
 }
 B200_API void b200_float8_tile_override(int tile) { float8::g_tile = tile; }

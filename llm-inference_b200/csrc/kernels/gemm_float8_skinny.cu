@@ -168,7 +168,23 @@ cudaError_t launch_kind(const SkinnyParams& p, int kind, dim3 grid, dim3 block, 
 
 }  // namespace
 
-int g_warps = 0;
+// All blocks run at once, 16 warps an SM (their registers), each warp with three slabs at least.
+static int skinny_warps(int N, int K) {
+  const int blocks = (N + kRows - 1) / kRows, slabs = (K + kSlabK - 1) / kSlabK, sms = b200_sm_count_host();
+  return max(1, min(kMostWarps / ((blocks + sms - 1) / sms), (slabs + 2) / 3));
+}
+
+// Streams that are short for a warp. Up to 8 tokens (us, this form and the streaming one): 2,048 x 1,536 2.3 and 4.3, 3,584 x 3,584 4.2 and 5.1, 4,608 x
+// 3,584 4.9 and 5.7 (7 slabs a warp), 5,120 x 5,120 8.2 and 7.2 (16). Up to 16, where a block takes as much of X as of W out of L2: 2,048 x 1,536
+// 2.9 and 4.3 (3 slabs), 896 x 4,864 4.5 and 5.5 (5), 3,584 x 3,584 6.3 and 5.5 (7).
+bool skinny_takes(int M, int N, int K) {
+  if (M > 16) return false;
+  const int blocks = (N + kRows - 1) / kRows, sms = b200_sm_count_host();
+  if (blocks > kMostWarps * sms) return false;
+  const int slabs = (K + kSlabK - 1) / kSlabK, warps = skinny_warps(N, K);
+  return (slabs + warps - 1) / warps <= (M <= 8 ? 9 : 5);
+}
+
 int launch_skinny(const Product& product, cudaStream_t stream) {
   SkinnyParams p;
   p.e = product.e;
@@ -178,9 +194,7 @@ int launch_skinny(const Product& product, cudaStream_t stream) {
   p.w_stride = product.w_stride;
   p.K = product.K;
   p.w_constant = product.w_constant;
-  const int slabs = (p.K + kSlabK - 1) / kSlabK;
-  int warps = g_warps > 0 ? g_warps : (slabs > 64 ? 16 : 8);
-  const dim3 grid((p.e.N + kRows - 1) / kRows), block(32 * warps);
+  const dim3 grid((p.e.N + kRows - 1) / kRows), block(32 * max(2, skinny_warps(p.e.N, p.K)));  // two: 64 threads finish
   cudaError_t status;
   if (p.e.M <= 8)
     status = product.out_f32 ? launch_kind<float, 1, 4>(p, product.kind, grid, block, stream) : launch_kind<__nv_bfloat16, 1, 4>(p, product.kind, grid, block, stream);
@@ -194,4 +208,3 @@ int launch_skinny(const Product& product, cudaStream_t stream) {
 }
 
 }  // namespace float8
-B200_API void b200_float8_warps(int w) { float8::g_warps = w; }

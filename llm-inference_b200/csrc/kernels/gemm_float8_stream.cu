@@ -353,39 +353,42 @@ int clusters_one_per_sm(int members) {
   return clusters;
 }
 
-struct Override { int stages = 0, members = 0, target = 0, budget = 0; };
+struct Override { int stages = 0, members = 0, budget = 0; };
 Override g_override;  // a sweep's (b200_float8_stream_override); zeros in normal use
 
-void size_ring(StreamPlan& plan, int k_blocks, bool f32) {
+// `budget`: bytes of shared memory that a block means to take.
+void size_ring(StreamPlan& plan, int k_blocks, bool f32, size_t budget) {
+  if (g_override.budget > 0) budget = static_cast<size_t>(g_override.budget) * 1024;
   const size_t stage = kRowsW * kBlockK + ((static_cast<size_t>(plan.tile) * kBlockK + 1023) & ~size_t(1023));
   const int per_block = (k_blocks + plan.members - 1) / plan.members;
-  // Accumulators: one, or one per chain where outputs are 32-bit, as many as fit.
+  size_t inbox = 0, outbox = 0;
+  if (plan.members > 1) {
+    const int slice = slice_rows(plan.members), owners = (kRowsW + slice - 1) / slice;
+    outbox = static_cast<size_t>(owners) * slice * plan.tile * sizeof(float);  // takes the ring's place
+    inbox = static_cast<size_t>(plan.members) * slice * plan.tile * sizeof(float);
+  }
+  const size_t for_ring = budget > inbox ? budget - inbox : 0;
+  plan.stages = max(2, min(min(static_cast<int>(for_ring / stage), kMaxStages), per_block));
+  if (g_override.stages > 0) plan.stages = g_override.stages;
+  const size_t ring = max(plan.stages * stage, outbox);
+  plan.inbox_at = static_cast<int>(ring);
+  plan.smem = ring + inbox + 1024;
+  // Accumulators: one, or one per chain where outputs are 32-bit, as many as the block's share of TMEM holds.
   const int wanted = f32 ? (per_block + kChainBlocks - 1) / kChainBlocks : 1;
-  const bool alone = wanted > 1 && wanted * plan.tile > 128 && plan.tile > 16;  // more than a quarter of TMEM: the SM to itself
-  const int most = alone ? 256 : 128;
+  const int most = budget > 114 * 1024 ? 256 : 128;
   const int accumulators = max(1, min(wanted, most / plan.tile));
   plan.chain_blocks = (per_block + accumulators - 1) / accumulators;
   plan.tmem_cols = 32;
   while (plan.tmem_cols < accumulators * plan.tile) plan.tmem_cols *= 2;
-  size_t budget = alone ? 190 * 1024 : (plan.blocks * plan.members * plan.tiles <= 2 * b200_sm_count_host() ? 100 * 1024 : 66 * 1024);
-  if (g_override.budget > 0) budget = static_cast<size_t>(g_override.budget) * 1024;
-  if (plan.members > 1) budget -= min(budget / 2, static_cast<size_t>(plan.members) * slice_rows(plan.members) * plan.tile * sizeof(float));  // the inbox
-  int stages = static_cast<int>(budget / stage);
-  if (g_override.stages > 0) stages = g_override.stages;
-  stages = min(min(stages, kMaxStages), per_block);
-  plan.stages = max(stages, 2);
-  size_t ring = plan.stages * stage, inbox = 0;
-  if (plan.members > 1) {
-    const int slice = slice_rows(plan.members), owners = (kRowsW + slice - 1) / slice;
-    ring = max(ring, static_cast<size_t>(owners) * slice * plan.tile * sizeof(float));  // the outbox takes its place
-    inbox = static_cast<size_t>(plan.members) * slice * plan.tile * sizeof(float);
-  }
-  plan.inbox_at = static_cast<int>(ring);
-  plan.smem = ring + inbox + 1024;
-  if (alone) plan.smem = max(plan.smem, static_cast<size_t>(118 * 1024));  // TMEM goes with shared memory: see the head of the file
-  else plan.smem = max(plan.smem, max(static_cast<size_t>(plan.tmem_cols) * 227 * 1024 / 512, static_cast<size_t>(48 * 1024)));
+  plan.smem = max(plan.smem, max(static_cast<size_t>(plan.tmem_cols) * 227 * 1024 / 512, static_cast<size_t>(48 * 1024)));  // see the head of the file
 }
 
+// Members share rows where there are too few blocks of 128 rows to give every SM one, as long as each keeps six or seven k-blocks to stream: below
+// that the sums cost more to bring together than the stream to share (48 tokens of 2,048 x 1,536: one member 4.7 us, four 5.6).
+// With more than 16 tokens a block has an SM to itself, and as many stages as that gives: two an SM hold fewer bytes in flight beside their inboxes (64
+// tokens of 17,920 x 1,536: 140 blocks 7.3 us, 280 of half the size 12.1; of 4,608 x 3,584: 108 blocks 8.4 us, 216 9.8). Up to 16 tokens
+// half again as many blocks as SMs (one of 4,608 x 3,584: 144 blocks 5.7 us, 216 6.2). All clusters should run at once: one that has to wait for a place
+// starts when the others are done, so clusters are narrowed until they do.
 StreamPlan plan_uncached(int M, int N, int K, bool f32) {
   StreamPlan plan;
   plan.blocks = (N + kRowsW - 1) / kRowsW;
@@ -394,27 +397,18 @@ StreamPlan plan_uncached(int M, int N, int K, bool f32) {
   const int k_blocks = (K + kBlockK - 1) / kBlockK;
   const int sms = b200_sm_count_host();
   const int columns = plan.blocks * plan.tiles;
-  int target = 2 * sms;
-  if (g_override.target > 0) target = g_override.target;
-  int widest = columns * 8 < sms ? kMaxMembers : 8;
-  if (g_override.members > 0) widest = g_override.members;
-  int members = max(1, min(widest, target / columns));
-  while (members > 1 && k_blocks / members < 2) --members;  // a block keeps a few stages to stream
-  members = min(members, k_blocks);
-  plan.members = members;
-  size_ring(plan, k_blocks, f32);
-  // All clusters should run at once: one that has to wait for a place starts when the others are done.
-  if (members > 1 && g_override.members <= 0) {
-    StreamPlan narrower = plan;
-    while (narrower.members > 1) {
-      const int per_sm = max(1, min(8, static_cast<int>((227 * 1024) / (narrower.smem + 3072))));
-      const int room = clusters_one_per_sm((narrower.members + per_sm - 1) / per_sm);
-      if (room == 0 || columns <= room) break;
-      --narrower.members;
-      size_ring(narrower, k_blocks, f32);
-    }
-    if (narrower.members > 1) plan = narrower;
-  }
+  const bool alone = plan.tile > 16 && columns <= sms;
+  auto fit = [&](int members, int per_sm) {  // a lower bound: s blocks an SM take clusters of m as one block an SM takes clusters of m / s
+    if (members == 1) return columns <= per_sm * sms;
+    const int room = clusters_one_per_sm((members + per_sm - 1) / per_sm);
+    return room == 0 || columns <= room;
+  };
+  plan.members = max(1, min(min(kMaxMembers, k_blocks / (plan.tile > 16 ? 7 : 6)), (alone ? sms : sms + sms / 2) / columns));
+  if (g_override.members > 0) plan.members = g_override.members;
+  else
+    while (plan.members > 1 && !fit(plan.members, alone ? 1 : 2)) --plan.members;
+  const bool one = alone || fit(plan.members, 1);
+  size_ring(plan, k_blocks, f32, (one ? (alone ? 190 : 150) : columns * plan.members <= 2 * sms ? 100 : 66) * 1024);
   return plan;
 }
 
@@ -427,7 +421,7 @@ StreamPlan plan_stream(int M, int N, int K, bool f32) {
   int device = 0;
   cudaGetDevice(&device);
   std::lock_guard<std::mutex> lock(guard);
-  if (g_override.stages > 0 || g_override.members > 0 || g_override.target > 0 || g_override.budget > 0) return plan_uncached(rows, N, K, f32);
+  if (g_override.stages > 0 || g_override.members > 0 || g_override.budget > 0) return plan_uncached(rows, N, K, f32);
   for (const Entry& e : known)
     if (e.m == rows && e.n == N && e.k == K && e.f32 == f32 && e.device == device) return e.plan;
   const StreamPlan plan = plan_uncached(rows, N, K, f32);
@@ -437,6 +431,19 @@ StreamPlan plan_stream(int M, int N, int K, bool f32) {
 }
 
 }  // namespace
+
+// Microseconds, roughly: a launch, bringing sums together, and the stream (a block's k-blocks one after the other, or what all of them take out of
+// L2 at 10 TB/s and out of memory at 6.5); fitted to 17 to 512 tokens of ten matrices.
+float stream_time(const Product& p) {
+  const StreamPlan plan = plan_stream(p.e.M, p.e.N, p.K, p.out_f32 != 0);
+  const int k_blocks = (p.K + kBlockK - 1) / kBlockK, sms = b200_sm_count_host();
+  const int columns = plan.blocks * plan.tiles;
+  const int turns = (columns * plan.members + sms - 1) / sms;
+  const float one = static_cast<float>((k_blocks + plan.members - 1) / plan.members) * turns * (0.1f + 0.001f * plan.tile);
+  const float all = static_cast<float>(columns) * k_blocks * (kRowsW + plan.tile) * kBlockK / 10e6f;
+  const float memory = static_cast<float>(p.e.N) * p.K / 6.5e6f;
+  return max((plan.members > 1 ? 4.5f + 0.028f * plan.tile : 3.6f) + max(one, all), 2.5f + memory);
+}
 
 int launch_stream(const Product& product, cudaStream_t stream) {
   const Epilogue& e = product.e;
@@ -490,6 +497,6 @@ int launch_stream(const Product& product, cudaStream_t stream) {
 }  // namespace float8
 
 // For parameter sweeps only: force the ring depth, the cluster width, the blocks aimed at or the ring's budget in KB (0: the planner's own).
-B200_API void b200_float8_stream_override(int stages, int members, int target, int budget) {
-  float8::g_override = {stages, members, target, budget};
+B200_API void b200_float8_stream_override(int stages, int members, int, int budget) {
+  float8::g_override = {stages, members, budget};
 }
