@@ -10,11 +10,10 @@
 // NaN stays NaN in its place (the largest magnitude is taken over the others); a row with an infinity has scale infinity, its finite numbers are
 // zeros and its infinities NaN, so what is made of that row is NaN and no other row is touched.
 //
-// Memory bound. A row's threads each hold kItems packs of eight numbers (16 bytes of bfloat16, two times 16 of 32 bits; 8 bytes of e4m3 out); rows whose length,
-// stride or base does not allow packs go a number at a time. A block takes as many rows as fit its threads, so short rows do not leave lanes
-// idle. Rows too long for the registers are read twice (the second time out of L2).
-#include <type_traits>
-
+// Memory bound. A row's threads each hold a few groups of 16 bytes (of single numbers where a row's length, stride or base does not allow that), all
+// asked for before the first is used. A block takes as many rows as fit its threads, so short rows do not leave lanes idle. Rows too long for
+// the registers are read twice, the second time out of L2. Of what memory takes at its copy rate: 8,192 rows of 3,584 with a bfloat16 branch output
+// 50.6 us of 49.3, 2,048 of 5,120 20.5 of 17.6.
 #include "float8.cuh"
 #include "packs.cuh"
 
@@ -27,45 +26,70 @@ __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {  // lo in th
   return r;
 }
 
-// Eight neighbouring numbers in packs, or one.
-template <int W>
-struct Group;
+// The larger magnitudes of two pairs of bfloat16 numbers (a NaN counts for nothing beside a number).
+__device__ __forceinline__ uint32_t max_abs(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
+  return r;
+}
+
+// W neighbouring numbers as they lie in memory, and as 32-bit ones.
+template <typename T, int W>
+struct Raw;
 template <>
-struct Group<8> {
-  float v[8];
-  template <typename T>
-  __device__ __forceinline__ void load(const T* p) {
-    const float4 a = load4<T>(p), b = load4<T>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  }
-  __device__ __forceinline__ void store(float* p) const {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  }
-  __device__ __forceinline__ void store_e4m3(uint8_t* p, float first, float second) const {
-    uint2 r;
-    r.x = to_e4m3x2(v[0] * first * second, v[1] * first * second) | to_e4m3x2(v[2] * first * second, v[3] * first * second) << 16;
-    r.y = to_e4m3x2(v[4] * first * second, v[5] * first * second) | to_e4m3x2(v[6] * first * second, v[7] * first * second) << 16;
-    *reinterpret_cast<uint2*>(p) = r;
+struct Raw<float, 4> {
+  float4 v;
+  __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ float largest() const { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }  // NaN counts for nothing
+  __device__ __forceinline__ void widen(float (&f)[4]) const { f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w; }
+};
+template <>
+struct Raw<__nv_bfloat16, 4> {
+  uint2 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ void widen(float (&f)[4]) const {
+    f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xffff0000u), f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xffff0000u);
   }
 };
 template <>
-struct Group<1> {
-  float v[1];
-  template <typename T>
-  __device__ __forceinline__ void load(const T* p) { v[0] = to_f32<T>(*p); }
-  __device__ __forceinline__ void store(float* p) const { *p = v[0]; }
-  __device__ __forceinline__ void store_e4m3(uint8_t* p, float first, float second) const { *p = static_cast<uint8_t>(to_e4m3x2(v[0] * first * second, 0.f)); }
-};
-template <>
-__device__ __forceinline__ void Group<8>::load<__nv_bfloat16>(const __nv_bfloat16* p) {
-  const uint4 raw = *reinterpret_cast<const uint4*>(p);
-  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+struct Raw<__nv_bfloat16, 8> {
+  uint4 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ float largest() const {  // two at a time
+    uint32_t m = max_abs(max_abs(v.x, v.y), max_abs(v.z, v.w));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  __device__ __forceinline__ void widen(float (&f)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(words[i] << 16);
-    v[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
+};
+template <typename T>
+struct Raw<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ float largest() const { return fabsf(to_f32<T>(v)); }
+  __device__ __forceinline__ void widen(float (&f)[1]) const { f[0] = to_f32<T>(v); }
+};
+__device__ __forceinline__ void store_f32(float* p, const float (&f)[4]) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+__device__ __forceinline__ void store_f32(float* p, const float (&f)[1]) { *p = f[0]; }
+__device__ __forceinline__ uint32_t four(const float* f, float factor) {
+  const float2 both = make_float2(factor, factor), lo = mul_2(make_float2(f[0], f[1]), both), hi = mul_2(make_float2(f[2], f[3]), both);
+  return to_e4m3x2(lo.x, lo.y) | to_e4m3x2(hi.x, hi.y) << 16;
+}
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[8], float factor) { *reinterpret_cast<uint2*>(p) = make_uint2(four(f, factor), four(f + 4, factor)); }
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[4], float factor) { *reinterpret_cast<uint32_t*>(p) = four(f, factor); }
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[1], float factor) { *p = static_cast<uint8_t>(to_e4m3x2(f[0] * factor, 0.f)); }
+// The same of a row that may need two factors (RowScale).
+template <int W>
+__device__ __forceinline__ void store_e4m3(uint8_t* p, float (&f)[W], float first, float second) {
+  if (second != 1.f) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) f[i] *= first;
+    first = second;
+  }
+  store_e4m3(p, f, first);
 }
 
 struct RowsParams {
@@ -81,165 +105,230 @@ struct RowsParams {
   float eps;
 };
 
-// Sum and maximum over a row's threads; `scratch` holds two floats a warp of the block.
-__device__ __forceinline__ void meet(float& sum, float& most, float2* scratch, int row_threads) {
+// Largest of numbers that are not negative (their bits are ordered as they are), and the sum too, over a row's threads; `scratch` holds a number a
+// warp of the block, each.
+__device__ __forceinline__ float warp_largest(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
+__device__ __forceinline__ float row_largest(float most, float* scratch, int row_threads) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  }
+  most = warp_largest(most);
+  if (row_threads == 32) return most;
+  const int warps = row_threads >> 5, first = warp / warps * warps;
+  if (lane == 0) scratch[warp] = most;
+  __syncthreads();
+  return warp_largest(lane < warps ? scratch[first + lane] : 0.f);
+}
+__device__ __forceinline__ void row_sum_and_largest(float& sum, float& most, float2* scratch, int row_threads) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  sum = warp_sum(sum);
+  most = warp_largest(most);
   if (row_threads == 32) return;
   const int warps = row_threads >> 5, first = warp / warps * warps;
   if (lane == 0) scratch[warp] = make_float2(sum, most);
   __syncthreads();
   const float2 part = lane < warps ? scratch[first + lane] : make_float2(0.f, 0.f);
-  sum = part.x;
-  most = part.y;
+  sum = warp_sum(part.x);
+  most = warp_largest(part.y);
+}
+
+constexpr float kSmallestAmax = kLargest * kSmallestScale;  // rows below it have the smallest scale
+
+// The factors of a normed row: what is held (before 1 / rms), times `first`, times `second`, is the quotient by the scale. 1 / rms cancels, 448 / most alone is
+// left, unless the row is so small that a factor would not be a normal number.
+struct RowScale {
+  float scale, first, second;
+  __device__ __forceinline__ RowScale(float most, float rstd) {
+    const float largest = most * rstd;
+    scale = largest < kSmallestAmax ? kSmallestScale : largest / kLargest;
+    if (most >= 1e-30f && largest >= kSmallestAmax) first = kLargest / most, second = 1.f;
+    else first = rstd, second = largest >= kSmallestAmax ? kLargest / largest : 1.f / kSmallestScale;
+  }
+};
+
+// W: numbers a group; ITEMS: groups a thread holds (0: the row is read twice instead); THREADS: of a block at most.
+template <typename T, int W, int ITEMS, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+float8_quantize_kernel(const RowsParams p) {
+  __shared__ float scratch[32];
+  const int in_block = blockDim.x / p.row_threads;
+  const int at_row = threadIdx.x / p.row_threads, t = threadIdx.x - at_row * p.row_threads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * in_block + at_row;
+  const bool live = row < p.rows;
+  const int groups = live ? p.columns / W : 0;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  uint8_t* out = p.out + row * p.out_stride;
+  wait_for_predecessor();
+  let_successor_start();
+  float most = 0.f;
+  Raw<T, W> held[ITEMS > 0 ? ITEMS : 1];
+  auto look = [&](const Raw<T, W>& g) { most = fmaxf(most, g.largest()); };
+  if constexpr (ITEMS > 0) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    for (int j = 0; j < ITEMS; ++j)
+      if (t + j * p.row_threads < groups) held[j].load(x + (t + j * p.row_threads) * W);
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (t + j * p.row_threads < groups) look(held[j]);
+  } else {
+    for (int at = t; at < groups; at += p.row_threads) {
+      held[0].load(x + at * W);
+      look(held[0]);
+    }
+  }
+  most = row_largest(most, scratch, p.row_threads);
+  if (!live) return;
+  if (t == 0) p.scales[row] = most >= kSmallestAmax ? most / kLargest : kSmallestScale;
+  const float factor = most >= kSmallestAmax ? kLargest / most : 1.f / kSmallestScale;
+  auto put = [&](const Raw<T, W>& g, int at) {
+    float f[W];
+    g.widen(f);
+    store_e4m3(out + at * W, f, factor);
+  };
+  if constexpr (ITEMS > 0) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (t + j * p.row_threads < groups) put(held[j], t + j * p.row_threads);
+  } else {
+    for (int at = t; at < groups; at += p.row_threads) {
+      held[0].load(x + at * W);
+      put(held[0], at);
+    }
   }
 }
 
-// W: numbers a group; ITEMS: groups a thread holds (0: the row is read twice instead).
-template <bool NORM, typename T, int W, int ITEMS>
-__global__ void __launch_bounds__(1024)
-float8_rows_kernel(const RowsParams p) {
+template <typename T, int W, int ITEMS, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+float8_rmsnorm_kernel(const RowsParams p) {
   __shared__ float2 scratch[32];
   const int in_block = blockDim.x / p.row_threads;
   const int at_row = threadIdx.x / p.row_threads, t = threadIdx.x - at_row * p.row_threads;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * in_block + at_row;
   const bool live = row < p.rows;
   const int groups = live ? p.columns / W : 0;
-  using Source = typename std::conditional<NORM, float, T>::type;
-  const Source* x = static_cast<const Source*>(p.x) + row * p.x_stride;
-  const T* delta = NORM && p.delta != nullptr ? static_cast<const T*>(p.delta) + row * p.delta_stride : nullptr;
-  float* stream = NORM && p.stream != nullptr ? p.stream + row * p.stream_stride : nullptr;
+  const float* x = static_cast<const float*>(p.x) + row * p.x_stride;
+  const T* delta = p.delta != nullptr ? static_cast<const T*>(p.delta) + row * p.delta_stride : nullptr;
+  float* stream = p.stream != nullptr ? p.stream + row * p.stream_stride : nullptr;
   uint8_t* out = p.out + row * p.out_stride;
+  constexpr int kHeld = ITEMS > 0 ? ITEMS : 1;
   // The weight depends on nothing on the stream: it is asked for first.
-  Group<W> weight[ITEMS > 0 ? ITEMS : 1];
-  if constexpr (NORM && ITEMS > 0) {
+  Raw<float, W> weight[kHeld];
+  if constexpr (ITEMS > 0) {
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j)
       if (t + j * p.row_threads < groups) weight[j].load(p.weight + (t + j * p.row_threads) * W);
   }
   wait_for_predecessor();
   let_successor_start();
-
   float sum = 0.f, most = 0.f;
-  auto fetch = [&](Group<W>& g, Group<W>& d, int at) {
-    g.load(x + at * W);
-    if (NORM && delta != nullptr) d.load(delta + at * W);
+  float held[kHeld][W];  // s w
+  Raw<float, W> from[kHeld];
+  Raw<T, W> added[kHeld];
+  auto fetch = [&](int j, int at) {
+    from[j].load(x + at * W);
+    if (delta != nullptr) added[j].load(delta + at * W);
   };
-  auto take = [&](Group<W>& g, const Group<W>& d, const Group<W>& w, int at) {  // a group's part of the sum and of the maximum; times w
-    if constexpr (NORM) {
-      if (delta != nullptr) {
+  auto take = [&](int j, int at, bool counts) {
+    float w[W];
+    from[j].widen(held[j]);
+    weight[j].widen(w);
+    if (delta != nullptr) {
+      float d[W];
+      added[j].widen(d);
 #pragma unroll
-        for (int i = 0; i < W; ++i) g.v[i] += d.v[i];
-      }
-      if (stream != nullptr) g.store(stream + at * W);
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        sum = fmaf(g.v[i], g.v[i], sum);
-        g.v[i] *= w.v[i];
-      }
+      for (int i = 0; i < W; ++i) held[j][i] += d[i];
     }
+    if (counts && stream != nullptr) store_f32(stream + at * W, held[j]);
 #pragma unroll
-    for (int i = 0; i < W; ++i) most = fmaxf(most, fabsf(g.v[i]));
+    for (int i = 0; i < W; ++i) {
+      sum = fmaf(held[j][i], held[j][i], sum);
+      held[j][i] *= w[i];
+      most = fmaxf(most, fabsf(held[j][i]));
+    }
   };
-  Group<W> held[ITEMS > 0 ? ITEMS : 1], added[ITEMS > 0 ? ITEMS : 1];
   if constexpr (ITEMS > 0) {
     // All loads first: the sum's stores may be to where the next group lies, as far as the compiler knows.
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j)
-      if (t + j * p.row_threads < groups) fetch(held[j], added[j], t + j * p.row_threads);
+      if (t + j * p.row_threads < groups) fetch(j, t + j * p.row_threads);
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j)
-      if (t + j * p.row_threads < groups) take(held[j], added[j], weight[j], t + j * p.row_threads);
+      if (t + j * p.row_threads < groups) take(j, t + j * p.row_threads, true);
   } else {
     for (int at = t; at < groups; at += p.row_threads) {
-      if constexpr (NORM) weight[0].load(p.weight + at * W);
-      fetch(held[0], added[0], at);
-      take(held[0], added[0], weight[0], at);
+      weight[0].load(p.weight + at * W);
+      fetch(0, at);
+      take(0, at, true);
     }
   }
-  meet(sum, most, scratch, p.row_threads);
+  row_sum_and_largest(sum, most, scratch, p.row_threads);
   if (!live) return;
-  // What is held, times `first`, times `second`, is the quotient by the scale. Of a normed row 1 / rms cancels: 448 / most alone, unless the row is so
-  // small that a factor would not be a normal number.
-  const float rstd = NORM ? rsqrtf(sum / static_cast<float>(p.columns) + p.eps) : 1.f;
-  const float largest = most * rstd;
-  float scale = largest / kLargest, first = rstd, second = 1.f / kSmallestScale;
-  if (scale >= kSmallestScale) {
-    first = most >= 1e-30f ? kLargest / most : rstd;
-    second = most >= 1e-30f ? 1.f : kLargest / largest;
-  }
-  if (scale < kSmallestScale) scale = kSmallestScale;
-  if (t == 0) p.scales[row] = scale;
+  const RowScale s(most, rsqrtf(sum / static_cast<float>(p.columns) + p.eps));
+  if (t == 0) p.scales[row] = s.scale;
   if constexpr (ITEMS > 0) {
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j)
-      if (t + j * p.row_threads < groups) held[j].store_e4m3(out + (t + j * p.row_threads) * W, first, second);
+      if (t + j * p.row_threads < groups) store_e4m3<W>(out + (t + j * p.row_threads) * W, held[j], s.first, s.second);
   } else {
-    // The second reading: of the sum where it was written out, else of its parts again.
+    // The second reading: of the sum where it was written (which may be where x was), else of its parts again.
+    if (stream != nullptr) x = stream, delta = nullptr;
     for (int at = t; at < groups; at += p.row_threads) {
-      if (NORM && stream != nullptr) {
-        held[0].load(stream + at * W);
-      } else {
-        held[0].load(x + at * W);
-        if (delta != nullptr) {
-          Group<W> d;
-          d.load(delta + at * W);
-#pragma unroll
-          for (int i = 0; i < W; ++i) held[0].v[i] += d.v[i];
-        }
-      }
-      if constexpr (NORM) {
-        weight[0].load(p.weight + at * W);
-#pragma unroll
-        for (int i = 0; i < W; ++i) held[0].v[i] *= weight[0].v[i];
-      }
-      held[0].store_e4m3(out + at * W, first, second);
+      weight[0].load(p.weight + at * W);
+      fetch(0, at);
+      take(0, at, false);
+      store_e4m3<W>(out + at * W, held[0], s.first, s.second);
     }
   }
 }
 
 bool aligned(const void* p, int64_t stride_bytes, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0 && stride_bytes % to == 0; }
 
-template <bool NORM, typename T, int W>
-cudaError_t launch_rows_as(RowsParams p, cudaStream_t stream) {
-  const int groups = p.columns / W;
-  constexpr int kMost = W == 8 ? 4 : 8;  // groups a thread holds
-  // Threads of a row: two groups each (one where rows are few, whose time is all latency), up to a block of 1,024.
-  const int each = W == 8 ? (p.rows >= 2 * b200_sm_count_host() ? 2 : 1) : 4;
-  int threads = ((groups + each - 1) / each + 31) / 32 * 32;
-  threads = max(32, min(threads, 1024));
-  int items = (groups + threads - 1) / threads;
-  // Short rows share a block of up to 256 threads, if there are enough of them to go round.
-  int in_block = 1;
-  while (threads * in_block * 2 <= 256 && p.rows >= 2 * in_block * 4 * b200_sm_count_host()) in_block *= 2;
-  p.row_threads = threads;
-  const dim3 grid((p.rows + in_block - 1) / in_block), block(threads * in_block);
-  if (items <= 1) return launch_kernel(float8_rows_kernel<NORM, T, W, 1>, grid, block, 0, stream, p);
-  if (items <= 2) return launch_kernel(float8_rows_kernel<NORM, T, W, 2>, grid, block, 0, stream, p);
-  if (items <= kMost) return launch_kernel(float8_rows_kernel<NORM, T, W, kMost>, grid, block, 0, stream, p);
-  return launch_kernel(float8_rows_kernel<NORM, T, W, 0>, grid, block, 0, stream, p);
+struct RowsShape {
+  int threads, in_block, items;
+};
+// Threads of a row, `each` groups a thread, up to a block of `most`. Short rows share a block of up to 256 threads, if there are enough of them to go round.
+RowsShape rows_shape(int rows, int groups, int each, int most) {
+  RowsShape s;
+  s.threads = max(32, min(most, ((groups + each - 1) / each + 31) / 32 * 32));
+  s.items = (groups + s.threads - 1) / s.threads;
+  s.in_block = 1;
+  while (s.threads * s.in_block * 2 <= 256 && rows >= 8 * s.in_block * b200_sm_count_host()) s.in_block *= 2;
+  return s;
 }
 
-template <bool NORM>
-int launch_rows(const RowsParams& p, bool packs, int dtype, cudaStream_t stream) {
-  cudaError_t status;
-  if (dtype == DTYPE_F32)
-    status = packs ? launch_rows_as<NORM, float, 8>(p, stream) : launch_rows_as<NORM, float, 1>(p, stream);
-  else
-    status = packs ? launch_rows_as<NORM, __nv_bfloat16, 8>(p, stream) : launch_rows_as<NORM, __nv_bfloat16, 1>(p, stream);
-  if (status != cudaSuccess) {
-    cudaGetLastError();
-    return b200_fail("float8 rows: %s", cudaGetErrorString(status));
-  }
-  return 0;
+template <typename Kernel>
+cudaError_t launch_shape(Kernel kernel, RowsParams p, const RowsShape& s, cudaStream_t stream) {
+  p.row_threads = s.threads;
+  return launch_kernel(kernel, dim3((p.rows + s.in_block - 1) / s.in_block), dim3(s.threads * s.in_block), 0, stream, p);
+}
+
+// Groups a thread: two where rows are few and all is latency (64 rows of 5,120: the norm with one group 3.1 us, with two 2.7); else four, of
+// eight bfloat16 numbers or of one number eight, so that what every thread does once a row counts less (1,777 rows of 1,001: 256 threads 5.9 us, 128 threads
+// 5.3). Longer rows are read twice (2,048 of 18,944 in 32 bits: 384 threads 39 us, 256 45).
+template <typename T, int W>
+cudaError_t launch_quantize(const RowsParams& p, cudaStream_t stream) {
+  const bool few = p.rows < 2 * b200_sm_count_host();
+  const RowsShape s = rows_shape(p.rows, p.columns / W, few && W > 1 ? 2 : W == 4 ? 4 : 8, few ? 1024 : 512);
+  if (s.items <= 1) return launch_shape(float8_quantize_kernel<T, W, 1, 1024>, p, s, stream);
+  if (s.items <= 2) return launch_shape(float8_quantize_kernel<T, W, 2, 1024>, p, s, stream);
+  if (s.items <= 4) return launch_shape(float8_quantize_kernel<T, W, 4, 1024>, p, s, stream);
+  if (s.items <= 8 && s.threads <= 512) return launch_shape(float8_quantize_kernel<T, W, 8, 512>, p, s, stream);
+  return launch_shape(float8_quantize_kernel<T, W, 0, 1024>, p, rows_shape(p.rows, p.columns / W, 1, few ? 1024 : 384), stream);
+}
+
+template <typename T, int W>
+cudaError_t launch_rmsnorm(const RowsParams& p, cudaStream_t stream) {
+  const bool few = p.rows < 2 * b200_sm_count_host();
+  const RowsShape s = rows_shape(p.rows, p.columns / W, W == 1 ? 8 : few ? 2 : 4, few ? 1024 : 512);
+  if (s.items <= 1) return launch_shape(float8_rmsnorm_kernel<T, W, 1, 1024>, p, s, stream);
+  if (s.items <= 2) return launch_shape(float8_rmsnorm_kernel<T, W, 2, 1024>, p, s, stream);
+  if (s.items <= 4 && s.threads <= 512) return launch_shape(float8_rmsnorm_kernel<T, W, 4, 512>, p, s, stream);
+  if (s.items <= 8 && s.threads <= 512) return launch_shape(float8_rmsnorm_kernel<T, W, 8, 512>, p, s, stream);
+  return launch_shape(float8_rmsnorm_kernel<T, W, 0, 1024>, p, s, stream);
+}
+
+int launched(cudaError_t status) {
+  if (status == cudaSuccess) return 0;
+  cudaGetLastError();
+  return b200_fail("float8 rows: %s", cudaGetErrorString(status));
 }
 
 }  // namespace
@@ -281,8 +370,10 @@ B200_API int b200_float8_quantize(const Float8Quantize* c, cudaStream_t stream) 
   p.x = c->x, p.x_stride = c->x_pitch, p.out = static_cast<uint8_t*>(c->out), p.out_stride = c->out_pitch, p.scales = c->scales;
   p.rows = static_cast<int>(c->rows), p.columns = static_cast<int>(c->columns);
   const int size = c->dtype == DTYPE_F32 ? 4 : 2;
-  const bool packs = p.columns % 8 == 0 && aligned(c->x, c->x_pitch * size, 16) && aligned(c->out, c->out_pitch, 8);
-  return launch_rows<false>(p, packs, static_cast<int>(c->dtype), stream);
+  const int w = 16 / size;  // numbers of 16 bytes
+  const bool packs = p.columns % w == 0 && aligned(c->x, c->x_pitch * size, 16) && aligned(c->out, c->out_pitch, w);
+  if (c->dtype == DTYPE_F32) return launched(packs ? launch_quantize<float, 4>(p, stream) : launch_quantize<float, 1>(p, stream));
+  return launched(packs ? launch_quantize<__nv_bfloat16, 8>(p, stream) : launch_quantize<__nv_bfloat16, 1>(p, stream));
 }
 
 B200_API int b200_float8_rmsnorm(const Float8RmsNorm* c, cudaStream_t stream) {
@@ -296,8 +387,9 @@ B200_API int b200_float8_rmsnorm(const Float8RmsNorm* c, cudaStream_t stream) {
   p.out = static_cast<uint8_t*>(c->out), p.out_stride = c->out_pitch, p.scales = c->scales;
   p.rows = static_cast<int>(c->rows), p.columns = static_cast<int>(c->columns);
   const int size = c->dtype == DTYPE_F32 ? 4 : 2;
-  const bool packs = p.columns % 8 == 0 && aligned(c->x, c->x_pitch * 4, 16) && aligned(c->weight, 0, 16) && aligned(c->out, c->out_pitch, 8) &&
-                     (c->delta == nullptr || aligned(c->delta, c->delta_pitch * size, 16)) &&
+  const bool packs = p.columns % 4 == 0 && aligned(c->x, c->x_pitch * 4, 16) && aligned(c->weight, 0, 16) && aligned(c->out, c->out_pitch, 4) &&
+                     (c->delta == nullptr || aligned(c->delta, c->delta_pitch * size, 4 * size)) &&
                      (c->stream == nullptr || aligned(c->stream, c->stream_pitch * 4, 16));
-  return launch_rows<true>(p, packs, static_cast<int>(c->dtype), stream);
+  if (c->dtype == DTYPE_F32) return launched(packs ? launch_rmsnorm<float, 4>(p, stream) : launch_rmsnorm<float, 1>(p, stream));
+  return launched(packs ? launch_rmsnorm<__nv_bfloat16, 4>(p, stream) : launch_rmsnorm<__nv_bfloat16, 1>(p, stream));
 }

@@ -433,14 +433,14 @@ StreamPlan plan_stream(int M, int N, int K, bool f32) {
 }  // namespace
 
 // Microseconds, roughly: a launch, bringing sums together, and the stream (a block's k-blocks one after the other, or what all of them take out of
-// L2 at 10 TB/s and out of memory at 6.5); fitted to 17 to 512 tokens of ten matrices.
+// L2 at 10 to 8 TB/s and out of memory at 6.5); fitted to 17 to 512 tokens of ten matrices.
 float stream_time(const Product& p) {
   const StreamPlan plan = plan_stream(p.e.M, p.e.N, p.K, p.out_f32 != 0);
   const int k_blocks = (p.K + kBlockK - 1) / kBlockK, sms = b200_sm_count_host();
   const int columns = plan.blocks * plan.tiles;
   const int turns = (columns * plan.members + sms - 1) / sms;
   const float one = static_cast<float>((k_blocks + plan.members - 1) / plan.members) * turns * (0.1f + 0.001f * plan.tile);
-  const float all = static_cast<float>(columns) * k_blocks * (kRowsW + plan.tile) * kBlockK / 10e6f;
+  const float all = static_cast<float>(columns) * k_blocks * (kRowsW + plan.tile) * kBlockK / (10.5e6f - 2e4f * plan.tile);
   const float memory = static_cast<float>(p.e.N) * p.K / 6.5e6f;
   return max((plan.members > 1 ? 4.5f + 0.028f * plan.tile : 3.6f) + max(one, all), 2.5f + memory);
 }
