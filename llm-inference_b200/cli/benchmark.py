@@ -138,7 +138,7 @@ def main(argv=None) -> int:
             "output_length": args.output_length if args.mix <= 0 else list(args.mix_output_lengths),
             "repetitions": args.repetitions, "concurrency": len(prompts),
             "prompt_token_lengths": [len(p) for p in prompts], "max_model_length": args.max_model_length,
-            "kv_cache_mib": args.kv_cache_mib, "stop_on_eos": args.stop_on_eos, "dtype": args.dtype,
+            "kv_cache_mib": args.kv_cache_mib, "stop_on_eos": args.stop_on_eos, "dtype": args.dtype, "weights": args.weights,
         },
         "aggregate": {
             "generated_tokens_per_second": sum(m["output_tokens"] for m in all_metrics) / seconds,

@@ -21,6 +21,8 @@ def add_engine_options(parser: argparse.ArgumentParser) -> None:
     parser.add_argument("--weights-seed", type=int, default=0, help="seed of --random's weights")
     parser.add_argument("--backend", choices=["auto", "cuda", "b200"], default="auto", help="kept from the reference's tools; this engine has one backend")
     parser.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    parser.add_argument("--weights", choices=["compute", "float8"], default="compute",
+                        help="'float8': the layers' projections in 8 bits (e4m3 with a scale a row), for architectures that have the form")
     parser.add_argument("--max-sequences", type=int, default=16)
     parser.add_argument("--max-model-length", type=int, default=2048)
     parser.add_argument("--kv-cache-mib", type=int, default=512)
@@ -43,7 +45,7 @@ def engine_from(args):
         dtype=args.dtype, max_num_sequences=args.max_sequences, max_model_length=args.max_model_length,
         kv_cache_bytes=args.kv_cache_mib << 20, page_size=args.page_size, prefill_chunk_size=args.prefill_chunk_size,
         prefill_burst_size=max(args.prefill_burst_size, args.prefill_chunk_size), cuda_graphs=not args.no_cuda_graphs,
-        run_ahead=not args.no_run_ahead, kernels=args.kernels, decode_kernel=args.decode_kernel, nvtx=args.nvtx, step_timing=args.step_timing,
+        weights=None if args.weights == "compute" else args.weights, run_ahead=not args.no_run_ahead, kernels=args.kernels, decode_kernel=args.decode_kernel, nvtx=args.nvtx, step_timing=args.step_timing,
     )
     if (args.model is None) == (args.random is None):
         raise SystemExit("give either --model DIR or --random SHAPE")
@@ -55,7 +57,7 @@ def engine_from(args):
         if args.random not in PRESETS:
             raise SystemExit(f"--random {args.random!r}: known shapes are {', '.join(sorted(PRESETS))}")
         _, config = parse_config(PRESETS[args.random])
-        options["model"] = random_model(config, seed=args.weights_seed, dtype=args.dtype)
+        options["model"] = random_model(config, seed=args.weights_seed, dtype=args.dtype, weights=options["weights"])
     return create_engine(args.model, backend=args.backend, **options)
 
 

@@ -24,7 +24,7 @@ from ..csrc.library import KernelError, check_error_word
 from ..parts.model import Model
 from ..sampling.params import GREEDY, SamplingParams
 from ..sampling.sampler import Sampler
-from .loading import load_model, parse_dtype
+from .loading import load_model, parse_dtype, parse_weights
 from .runner import ModelRunner, StepEntry
 
 PAGE_SIZE = 64
@@ -94,6 +94,7 @@ class Engine:
         max_batch_tokens: int | None = None,
         page_size: int = PAGE_SIZE,
         dtype: str | torch.dtype = "bfloat16",
+        weights: str | None = None,
         device: str | torch.device = "cuda:0",
         seed: int = 0,
         num_pages: int | None = None,
@@ -119,9 +120,14 @@ class Engine:
         if model is None:
             if model_path is None:
                 raise ValueError("give the engine a model folder (config.json plus safetensors)")
-            model = load_model(model_path, dtype, device)
+            # weights="float8": the layers' projections in e4m3 with a scale a row (half the bytes of a decode step's weights).
+            model = load_model(model_path, dtype, device, weights)
         elif model.device is None:
             raise ValueError("the model's weights are not loaded")
+        elif parse_weights(weights) not in (None, model.weights):
+            raise ValueError(f"weights={weights!r}, but the given model holds its weights in {model.weights or 'its compute dtype'}")
+        if kernels == "plain" and model.weights == "float8":
+            raise ValueError("weights in 8 bits have no plain kernels: use kernels='tuned'")
         self.model = model
         self.device = model.device
         self.dtype = parse_dtype(model.dtype)

@@ -33,9 +33,17 @@ def parse_dtype(dtype: str | torch.dtype) -> torch.dtype:
         raise ValueError(f"unknown dtype {dtype!r}; use 'bfloat16' or 'float32'") from None
 
 
-def load_model(model_path: str | Path, dtype: str | torch.dtype = "bfloat16", device: str | torch.device = "cuda:0") -> Model:
-    """Build the model that ``config.json`` names and load its safetensors weights."""
-    compute_dtype = parse_dtype(dtype)
+def parse_weights(weights: str | None) -> str | None:
+    """How the layers' projections are held: None in the compute dtype, ``"float8"`` in e4m3 with a scale a row."""
+    if weights in (None, "float8"):
+        return weights
+    raise ValueError(f"unknown weights {weights!r}; use None (the compute dtype) or 'float8'")
+
+
+def load_model(model_path: str | Path, dtype: str | torch.dtype = "bfloat16", device: str | torch.device = "cuda:0", weights: str | None = None) -> Model:
+    """Build the model that ``config.json`` names and load its safetensors weights; with ``weights="float8"`` the layers' projections are
+    then held in 8 bits (:meth:`Model.to_float8`)."""
+    compute_dtype, weights = parse_dtype(dtype), parse_weights(weights)
     folder = Path(model_path)
     if not folder.is_dir():
         raise FileNotFoundError(f"{folder} is not a model folder (config.json plus *.safetensors)")
@@ -43,6 +51,8 @@ def load_model(model_path: str | Path, dtype: str | torch.dtype = "bfloat16", de
     model = Model(entry.recipe(config))
     tensors = load_weights(folder, model.tensor_specs(), device="cpu")
     model.load(tensors, compute_dtype, torch.device(device))
+    if weights == "float8":
+        model.to_float8()
     return model
 
 
@@ -53,11 +63,14 @@ def random_model(
     device: str | torch.device = "cuda:0",
     *,
     std: float = 0.02,
+    weights: str | None = None,
 ) -> Model:
     """A model with seeded random weights drawn straight on the device (nothing is written)."""
     entry = resolve_architecture(config.to_json_dict())
     model = Model(entry.recipe(config))
-    dt = parse_dtype(dtype)
+    dt, weights = parse_dtype(dtype), parse_weights(weights)
     tensors = random_weights(model.tensor_specs(), seed, std=std, dtype=torch.bfloat16, device=device)
     model.load(tensors, dt, torch.device(device))
+    if weights == "float8":
+        model.to_float8()
     return model

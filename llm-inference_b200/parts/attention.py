@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from ..weights.loader import TensorSpec
-from . import ops
+from . import float8, ops
 from .base import KVCacheSpec, Part, PartSpec, build_part, register_part
 from .context import CacheView, StepContext
 
@@ -70,14 +70,22 @@ class GroupedQueryAttention(Part):
         self.w_o = tensors[f"{p}o_proj.weight"].to(device=device, dtype=dtype).contiguous()
         self.position.load(tensors, dtype, device)
 
+    def to_float8(self) -> None:
+        self.w_qkv, self.w_o, self.float8 = float8.from_tensor(self.w_qkv), float8.from_tensor(self.w_o), True
+
     def weight_bytes(self) -> int:
+        if self.float8:
+            return self.w_qkv.bytes() + self.w_o.bytes() + (self.b_qkv.numel() * 4 if self.b_qkv is not None else 0)
         total = self.w_qkv.numel() * self.w_qkv.element_size() + self.w_o.numel() * self.w_o.element_size()
         return total + (self.b_qkv.numel() * 4 if self.b_qkv is not None else 0)
 
     takes_folded = True  # `h` may be ops.FoldedRows: the q/k/v product applies the norm's 1 / rms
     takes_sink = True  # with a sink the output product adds into the residual stream itself
+    float8 = False  # projections in 8 bits: `h` is then float8.Float8Rows
 
     def forward(self, ctx: StepContext, cache: CacheView, h, sink: ops.ResidualSink | None = None):
+        if self.float8:
+            return self._forward_float8(ctx, cache, h)
         t = ctx.num_tokens
         width = (self.q_heads + 2 * self.kv_heads) * self.head_dim
         qkv = ops.linear(ctx, h, self.w_qkv, ctx.buffer("qkv", (t, width)))
@@ -92,6 +100,17 @@ class GroupedQueryAttention(Part):
             if folded is not None:
                 return folded
         return ops.linear(ctx, attn, self.w_o, ctx.buffer("branch", (t, self.hidden_size)))
+
+    def _forward_float8(self, ctx: StepContext, cache: CacheView, h: float8.Float8Rows) -> torch.Tensor:
+        t, inner = ctx.num_tokens, self.q_heads * self.head_dim
+        width = inner + 2 * self.kv_heads * self.head_dim
+        qkv = float8.linear(ctx, h, self.w_qkv, ctx.buffer("qkv", (t, width)), bias=self.b_qkv)
+        q = ctx.buffer("q", (t, inner))
+        self.position.apply(ctx, cache, qkv, None, q, self.q_heads, self.kv_heads, self.head_dim)
+        attn = ctx.buffer("attn", (t, inner))
+        self.attend(ctx, cache, q, attn)
+        rows = float8.quantize(ctx, attn, float8.buffer_rows(ctx, "attn8", t, inner))
+        return float8.linear(ctx, rows, self.w_o, ctx.buffer("branch", (t, self.hidden_size)))
 
     def attend(self, ctx: StepContext, cache: CacheView, q: torch.Tensor, out: torch.Tensor) -> None:
         from . import attention_dispatch

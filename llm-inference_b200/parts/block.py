@@ -46,8 +46,24 @@ class PreNormResidualBlock(Part):
     def cache_spec(self):
         return self.mixer.cache_spec()
 
+    def float8_refusal(self) -> str | None:
+        """Why this layer's projections cannot be in 8 bits, or None."""
+        for kind, part, method in (("mixer", self.mixer, "to_float8"), ("feed-forward", self.feed_forward, "to_float8"),
+                                   ("norm", self.mixer_norm, "forward_float8"), ("norm", self.feed_forward_norm, "forward_float8")):
+            if not hasattr(part, method):
+                return f"its {kind} {type(part).__name__} has no form for them"
+        return None
+
+    def to_float8(self) -> None:
+        """Both sublayers' matrices in 8 bits, and the norms' outputs with them."""
+        self.mixer.to_float8()
+        self.feed_forward.to_float8()
+
     def forward(self, ctx: StepContext, cache: CacheView | None, x: torch.Tensor, delta, next_norm: Part | None = None):
         mixer, ff = self.mixer, self.feed_forward
+        if getattr(mixer, "float8", False):
+            a = mixer.forward(ctx, cache, self.mixer_norm.forward_float8(ctx, x, delta))
+            return ff.forward(ctx, self.feed_forward_norm.forward_float8(ctx, x, a))
         h = self._norm(self.mixer_norm, ctx, x, delta, getattr(mixer, "takes_folded", False))
         # The mixer's and the feed-forward's outputs share one scratch buffer: the second norm
         # has consumed the former before the feed-forward's last product writes the latter.

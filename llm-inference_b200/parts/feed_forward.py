@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from ..weights.loader import TensorSpec
-from . import ops
+from . import float8, ops
 from .base import Part, register_part
 from .context import StepContext
 
@@ -37,14 +37,24 @@ class SwiGLU(Part):
         self.w_gate_up = torch.stack([gate, up], dim=1).reshape(2 * self.intermediate_size, self.hidden_size).contiguous()
         self.w_down = tensors[p + self.names[2]].to(device=device, dtype=dtype).contiguous()
 
+    def to_float8(self) -> None:
+        self.w_gate_up, self.w_down, self.float8 = float8.from_tensor(self.w_gate_up), float8.from_tensor(self.w_down), True
+
     def weight_bytes(self) -> int:
+        if self.float8:
+            return self.w_gate_up.bytes() + self.w_down.bytes()
         return (self.w_gate_up.numel() + self.w_down.numel()) * self.w_down.element_size()
 
     takes_folded = True  # `h` may be ops.FoldedRows: the gate/up product applies the norm's 1 / rms
     takes_sink = True  # with a sink the down product adds into the residual stream itself
+    float8 = False  # matrices in 8 bits: `h` is then float8.Float8Rows
 
     def forward(self, ctx: StepContext, h, sink: ops.ResidualSink | None = None):
         t, i = ctx.num_tokens, self.intermediate_size
+        if self.float8:
+            act = float8.linear_gated(ctx, h, self.w_gate_up, ctx.buffer("act", (t, i)), self.activation)
+            rows = float8.quantize(ctx, act, float8.buffer_rows(ctx, "act8", t, i))
+            return float8.linear(ctx, rows, self.w_down, ctx.buffer("branch", (t, self.hidden_size)))
         act = ctx.buffer("act", (t, i))
         if not ops.linear_gated(ctx, h, self.w_gate_up, act, self.activation):
             gate_up = ops.linear(ctx, h, self.w_gate_up, ctx.buffer("gate_up", (t, 2 * i)))

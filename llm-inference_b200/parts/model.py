@@ -85,6 +85,7 @@ class Model:
                 raise ValueError(f"the run order names layer {call.layer}, which does not exist")
         self.dtype: torch.dtype | None = None
         self.device: torch.device | None = None
+        self.weights: str | None = None  # "float8" after `to_float8`
         self._ids = None
         self.graph_safe = all(
             p.graph_safe for p in (self.embedding, *self.blocks, self.final_norm, self.head)
@@ -105,11 +106,26 @@ class Model:
 
     def load(self, tensors: dict[str, torch.Tensor], dtype: torch.dtype, device: torch.device | str) -> None:
         device = torch.device(device)
-        self.dtype, self.device = dtype, device
+        self.dtype, self.device, self.weights = dtype, device, None
         for part in (self.embedding, *self.blocks, self.final_norm, self.head):
             part.load(tensors, dtype, device)
         if hasattr(self.head, "share"):
             self.head.share(self.embedding)
+
+    def to_float8(self) -> None:
+        """Every layer's projections in e4m3 with a scale a row, laid out once from the loaded weights; embedding, norms and head stay as they are.
+        ``ValueError`` for a model that is not in bfloat16 or has a layer without such a form."""
+        if self.weights == "float8":
+            return
+        if self.dtype != torch.bfloat16:
+            raise ValueError(f"weights in 8 bits need a model that computes in bfloat16, not {self.dtype}")
+        for index, block in enumerate(self.blocks):
+            refusal = block.float8_refusal() if hasattr(block, "float8_refusal") else f"its arrangement {type(block).__name__} has no form for them"
+            if refusal is not None:
+                raise ValueError(f"layer {index} cannot have its weights in 8 bits: {refusal}")
+        for block in self.blocks:
+            block.to_float8()
+        self.weights = "float8"
 
     def weight_bytes(self) -> int:
         """Bytes of weights a step reads: every layer call's weights, the last norm, the head."""

@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from ..weights.loader import TensorSpec
-from . import ops
+from . import float8, ops
 from .base import Part, register_part
 from .context import StepContext
 
@@ -53,6 +53,10 @@ class RMSNorm(Part):
         count = x.shape[0] if rows is None else rows.shape[0]
         out = ctx.buffer(out_name, (count, self.hidden_size), per_token=rows is None)
         return ops.rmsnorm(ctx, x, delta, self.weight, self.eps, out, rows)
+
+    def forward_float8(self, ctx: StepContext, x: torch.Tensor, delta: torch.Tensor | None) -> float8.Float8Rows:
+        """The same with its rows in 8 bits, the operand of a product with 8-bit weights."""
+        return float8.rmsnorm(ctx, x, delta, self.weight, self.eps, float8.buffer_rows(ctx, "normed8", x.shape[0], self.hidden_size))
 
 
 class GroupedRMSNorm(Part):

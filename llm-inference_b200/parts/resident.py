@@ -95,7 +95,7 @@ class ResidentDecoder:
             if type(block) is not PreNormResidualBlock:
                 return None
             mixer, ff = block.mixer, block.feed_forward
-            if type(mixer) is not GroupedQueryAttention or type(ff) is not SwiGLU:
+            if type(mixer) is not GroupedQueryAttention or type(ff) is not SwiGLU or mixer.float8 or ff.float8:
                 return None
             if type(block.mixer_norm) is not RMSNorm or type(block.feed_forward_norm) is not RMSNorm:
                 return None
