@@ -359,7 +359,7 @@ struct Float8RmsNorm {
 };
 static_assert(sizeof(Float8Quantize) == 8 * 8 && sizeof(Float8RmsNorm) == 14 * 8, "as packed by the caller");
 
-static bool float8_sizes(int64_t rows, int64_t columns) { return rows > 0 && columns > 0 && rows < (int64_t(1) << 31) && columns < (int64_t(1) << 31); }
+static bool float8_sizes(int64_t rows, int64_t columns) { return rows > 0 && columns > 0 && rows <= (int64_t(1) << 30) && columns <= (int64_t(1) << 30); }
 
 B200_API int b200_float8_quantize(const Float8Quantize* c, cudaStream_t stream) {
   using namespace float8;

@@ -3,7 +3,6 @@
 
 namespace float8 {
 
-int g_tile = 0;
 namespace {
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -72,7 +71,7 @@ static_assert(sizeof(Float8Linear) == 19 * 8, "as packed by the caller");
 B200_API int b200_float8_linear(const Float8Linear* c, cudaStream_t stream) {
   using namespace float8;
   if (c->M == 0 || c->N == 0) return 0;
-  constexpr int64_t kMost = (int64_t(1) << 31) - 1;
+  constexpr int64_t kMost = int64_t(1) << 30;  // counts and coordinates are 32-bit
   B200_REQUIRE(c->M > 0 && c->N > 0 && c->K > 0 && c->M <= kMost && c->N <= kMost && c->K <= kMost, "float8 product: bad sizes");
   Product p;
   p.x = c->x, p.w = c->w, p.x_stride = c->x_pitch, p.w_stride = c->w_pitch, p.K = static_cast<int>(c->K);
@@ -93,9 +92,9 @@ B200_API int b200_float8_linear(const Float8Linear* c, cudaStream_t stream) {
   const int size = p.out_f32 ? 4 : 2, at_once = p.kind == GATED ? 2 : 4;  // outputs from four rows of W
   e.vector = e.out_stride % at_once == 0 && reinterpret_cast<uintptr_t>(e.out) % (at_once * size) == 0 &&
              (e.residual == nullptr || (e.residual_stride % 4 == 0 && reinterpret_cast<uintptr_t>(e.residual) % 16 == 0));
-  if (g_tile == -1) return launch_skinny(p, stream);
-  if (g_tile == -2) return launch_stream(p, stream);
-  if (g_tile > 0) return launch_tiles(p, g_tile, stream);
-  return launch_chosen(p, stream);
+  try {
+    return launch_chosen(p, stream);
+  } catch (...) {  // plans are kept in containers
+    return b200_fail("float8 product: out of memory on the host");
+  }
 }
-B200_API void b200_float8_tile_override(int tile) { float8::g_tile = tile; }

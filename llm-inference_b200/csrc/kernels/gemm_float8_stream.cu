@@ -8,7 +8,7 @@
 // order, so a sum does not depend on timing. A block puts its sums where its ring was, one bulk copy per owner takes them to an inbox behind the
 // owner's ring, and the owner waits for the bytes: nobody waits for a member that has nothing to do with its rows, and the cluster meets only to
 // know that barriers are there and, on leaving, that copies have been read. (64 tokens of 4,608 x 3,584: 11.1 us with the cluster meeting
-// three times and single stores into neighbours' memory, TIME_BULK so.)
+// three times and single stores into neighbours' memory, 8.0 so.)
 //
 // 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as TMEM goes, added up as they are read.
 //
@@ -17,7 +17,9 @@
 // front before it, the second block of every SM began 2.7 us late, with it in front 1.1 us). A block takes no larger a share of an SM's TMEM than of its
 // shared memory, so a resident block never waits for another's. Every wait is bounded: a block that gives up sets the timeout bit, waits for its
 // copies in flight, frees its TMEM and leaves.
+#include <map>
 #include <mutex>
+#include <tuple>
 #include <vector>
 
 #include "float8.cuh"
@@ -353,12 +355,8 @@ int clusters_one_per_sm(int members) {
   return clusters;
 }
 
-struct Override { int stages = 0, members = 0, budget = 0; };
-Override g_override;  // a sweep's (b200_float8_stream_override); zeros in normal use
-
 // `budget`: bytes of shared memory that a block means to take.
 void size_ring(StreamPlan& plan, int k_blocks, bool f32, size_t budget) {
-  if (g_override.budget > 0) budget = static_cast<size_t>(g_override.budget) * 1024;
   const size_t stage = kRowsW * kBlockK + ((static_cast<size_t>(plan.tile) * kBlockK + 1023) & ~size_t(1023));
   const int per_block = (k_blocks + plan.members - 1) / plan.members;
   size_t inbox = 0, outbox = 0;
@@ -369,7 +367,6 @@ void size_ring(StreamPlan& plan, int k_blocks, bool f32, size_t budget) {
   }
   const size_t for_ring = budget > inbox ? budget - inbox : 0;
   plan.stages = max(2, min(min(static_cast<int>(for_ring / stage), kMaxStages), per_block));
-  if (g_override.stages > 0) plan.stages = g_override.stages;
   const size_t ring = max(plan.stages * stage, outbox);
   plan.inbox_at = static_cast<int>(ring);
   plan.smem = ring + inbox + 1024;
@@ -404,30 +401,25 @@ StreamPlan plan_uncached(int M, int N, int K, bool f32) {
     return room == 0 || columns <= room;
   };
   plan.members = max(1, min(min(kMaxMembers, k_blocks / (plan.tile > 16 ? 7 : 6)), (alone ? sms : sms + sms / 2) / columns));
-  if (g_override.members > 0) plan.members = g_override.members;
-  else
-    while (plan.members > 1 && !fit(plan.members, alone ? 1 : 2)) --plan.members;
+  while (plan.members > 1 && !fit(plan.members, alone ? 1 : 2)) --plan.members;
   const bool one = alone || fit(plan.members, 1);
   size_ring(plan, k_blocks, f32, (one ? (alone ? 190 : 150) : columns * plan.members <= 2 * sms ? 100 : 66) * 1024);
   return plan;
 }
 
-// Plans are remembered: the occupancy question costs more than a launch. A plan goes by N, K and the padded tokens only.
+// Plans are remembered: the occupancy question costs more than a launch. A plan goes by N, K, the padded tokens and the outputs' type only.
 StreamPlan plan_stream(int M, int N, int K, bool f32) {
-  struct Entry { int m, n, k; bool f32; int device; StreamPlan plan; };
   static std::mutex guard;
-  static std::vector<Entry> known;
-  const int rows = (M + 15) / 16 * 16;
+  static std::map<std::tuple<int, int, int, bool, int>, StreamPlan> known;
   int device = 0;
   cudaGetDevice(&device);
+  const int rows = (M + 15) / 16 * 16;
+  const auto key = std::make_tuple(N, K, rows, f32, device);
   std::lock_guard<std::mutex> lock(guard);
-  if (g_override.stages > 0 || g_override.members > 0 || g_override.budget > 0) return plan_uncached(rows, N, K, f32);
-  for (const Entry& e : known)
-    if (e.m == rows && e.n == N && e.k == K && e.f32 == f32 && e.device == device) return e.plan;
-  const StreamPlan plan = plan_uncached(rows, N, K, f32);
-  if (known.size() >= 4096) known.clear();
-  known.push_back({rows, N, K, f32, device, plan});
-  return plan;
+  const auto found = known.find(key);
+  if (found != known.end()) return found->second;
+  if (known.size() >= 8192) known.clear();
+  return known[key] = plan_uncached(rows, N, K, f32);
 }
 
 }  // namespace
@@ -495,8 +487,3 @@ int launch_stream(const Product& product, cudaStream_t stream) {
 }
 
 }  // namespace float8
-
-// For parameter sweeps only: force the ring depth, the cluster width, the blocks aimed at or the ring's budget in KB (0: the planner's own).
-B200_API void b200_float8_stream_override(int stages, int members, int, int budget) {
-  float8::g_override = {stages, members, budget};
-}

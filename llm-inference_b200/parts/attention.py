@@ -68,6 +68,7 @@ class GroupedQueryAttention(Part):
                 [tensors[f"{p}{n}.bias"].to(device=device, dtype=torch.float32) for n in names]
             ).contiguous()
         self.w_o = tensors[f"{p}o_proj.weight"].to(device=device, dtype=dtype).contiguous()
+        self.float8 = False
         self.position.load(tensors, dtype, device)
 
     def to_float8(self) -> None:

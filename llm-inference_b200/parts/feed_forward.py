@@ -36,6 +36,7 @@ class SwiGLU(Part):
         gate, up = (tensors[p + n].to(device=device, dtype=dtype) for n in self.names[:2])
         self.w_gate_up = torch.stack([gate, up], dim=1).reshape(2 * self.intermediate_size, self.hidden_size).contiguous()
         self.w_down = tensors[p + self.names[2]].to(device=device, dtype=dtype).contiguous()
+        self.float8 = False
 
     def to_float8(self) -> None:
         self.w_gate_up, self.w_down, self.float8 = float8.from_tensor(self.w_gate_up), float8.from_tensor(self.w_down), True

@@ -19,6 +19,7 @@ from .context import StepContext
 LARGEST = 448.0  # of e4m3
 SMALLEST_SCALE = 2.0**-126
 ROW_BYTES = 16  # rows start on multiples of this
+MOST = 2**30  # rows, columns
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "squared_relu": 3}  # gelu in its tanh form
 GATED_ACTIVATIONS = ("silu", "gelu")
@@ -60,7 +61,7 @@ def buffer_rows(ctx: StepContext, name: str, rows: int, columns: int) -> Float8R
 
 
 def from_tensor(weight: torch.Tensor) -> Float8Rows:
-    """A weight matrix in 8 bits, laid out once (torch operations on the weight's own device; nothing of a step)."""
+    """A weight matrix in 8 bits, laid out once, before any step: torch operations on the weight's own device, which have ended when this returns."""
     if weight.dim() != 2:
         raise KernelError(f"float8: a matrix has two dimensions, not {weight.dim()}")
     out = empty_rows(*weight.shape, weight.device)
@@ -69,6 +70,8 @@ def from_tensor(weight: torch.Tensor) -> Float8Rows:
         scales = torch.clamp(rows.abs().amax(1) / LARGEST, min=SMALLEST_SCALE) if rows.shape[1] else torch.full_like(out.scales[at : at + 4096], SMALLEST_SCALE)
         out.scales[at : at + 4096] = scales
         out.values[at : at + 4096] = (rows / scales[:, None]).clamp(-LARGEST, LARGEST).to(torch.float8_e4m3fn)
+    if weight.is_cuda:
+        torch.cuda.current_stream(weight.device).synchronize()
     out.constant = True
     return out
 
@@ -104,9 +107,9 @@ def _rows(name: str, m: Float8Rows, index: int) -> tuple[int, int, int, int, int
             pitch = -(-columns // ROW_BYTES) * ROW_BYTES
         address = v.data_ptr()
         if (v.dtype is _E4M3 and (step == 1 or columns <= 1) and not (address | pitch) % ROW_BYTES and pitch >= columns and v.get_device() == index
-                and s.dtype is _F32 and s.shape == (rows,) and (rows <= 1 or s.stride(0) == 1) and s.get_device() == index and rows < 2**31 and columns < 2**31):
+                and s.dtype is _F32 and s.shape == (rows,) and (rows <= 1 or s.stride(0) == 1) and s.get_device() == index and rows <= MOST and columns <= MOST):
             return address, pitch, s.data_ptr(), rows, columns
-    raise KernelError(f"float8: {name} must be e4m3 [rows, columns] whose rows are contiguous on 16-byte boundaries, with float32 [rows] scales, on "
+    raise KernelError(f"float8: {name} must be e4m3 [rows, columns] whose rows are contiguous on 16-byte boundaries, with float32 [rows] scales, at most 2**30 of each, on "
                       f"{_device_name(index)}; got {v.dtype} {list(v.shape)} (strides {list(v.stride())}, {v.device}) and {s.dtype} {list(s.shape)} ({s.device})")
 
 

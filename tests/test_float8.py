@@ -361,6 +361,88 @@ def test_weights_made_on_the_same_stream_are_waited_for(lib):
         assert torch.equal(out, want[turn % 2])
 
 
+@gpu
+@pytest.mark.parametrize("constant", [True, False])
+@pytest.mark.parametrize("m,n,k", [(3, 336, 1200), (50, 400, 2320), (40, 17936, 1040), (900, 1056, 720)])
+def test_first_call_of_a_size_inside_a_capture(lib, m, n, k, constant):
+    """Plans and attributes are made then; nothing of that is a stream's work."""
+    torch.manual_seed(17)
+    x, w = operand(m, k), operand(n, k, 0.05)
+    w.constant = constant
+    ctx = make_ctx(lib, positions=[0])
+    out = torch.zeros(m, n, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ctx.stream = torch.cuda.current_stream().cuda_stream
+        float8.linear(ctx, x, w, out)
+    graph.replay()
+    torch.cuda.synchronize()
+    y, magnitudes = wide_product(x, w)
+    assert torch.all((out.double() - y).abs() <= sum_off(k, magnitudes, torch.float32) + half_step(torch.float32) * 1.01 * y.abs())
+
+
+@gpu
+def test_threads_of_one_process(lib):
+    """Two threads, streams and sets of sizes at once."""
+    import threading
+
+    torch.manual_seed(18)
+    cases = [[(m, operand(m, 640), operand(n, 640, 0.05)) for m, n in sizes] for sizes in (((1, 512), (40, 1024), (300, 768)), ((2, 528), (70, 1040), (600, 512)))]
+    want = [[float8.linear(make_ctx(lib, positions=[0]), x, w, torch.empty(m, w.shape[0], device="cuda")) for m, x, w in case] for case in cases]
+    torch.cuda.synchronize()
+    wrong: list = []
+
+    def work(case, expected):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            ctx = make_ctx(lib, positions=[0])
+            for _ in range(30):
+                got = [float8.linear(ctx, x, w, torch.empty(m, w.shape[0], device="cuda")) for m, x, w in case]
+            stream.synchronize()
+            wrong.extend(not torch.equal(a, b) for a, b in zip(got, expected))
+
+    threads = [threading.Thread(target=work, args=pair) for pair in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(wrong) == 6 and not any(wrong)
+
+
+@gpu
+def test_offsets_past_32_bits(lib):
+    """Rows whose numbers lie more than 2^31 elements behind the first: the last rows and columns of each are right."""
+    torch.manual_seed(19)
+    ctx = make_ctx(lib, positions=[0])
+    rows, columns = 120000, 18944
+    x = torch.empty(rows, columns, device="cuda", dtype=torch.bfloat16)
+    x[-300:] = torch.randn(300, columns, device="cuda").bfloat16()
+    x[:-300] = 0.5
+    out = float8.quantize(ctx, x, float8.empty_rows(rows, columns, "cuda:0"))
+    check_rows(float8.Float8Rows(out.values[-300:], out.scales[-300:]), x[-300:].double(), 2.0**-23, 2.0**-22)
+    del x
+    # That matrix as the weights of a few tokens, and as many tokens of a small product whose outputs pass 2^31 too.
+    out.constant = True
+    few = operand(3, columns)
+    y = float8.linear(ctx, few, out, torch.empty(3, rows, device="cuda"))
+    last = float8.Float8Rows(out.values[-300:], out.scales[-300:])
+    want, magnitudes = wide_product(few, last)
+    assert torch.all((y[:, -300:].double() - want).abs() <= sum_off(columns, magnitudes, torch.float32) + half_step(torch.float32) * 1.01 * want.abs())
+    del out, y
+    many, w = operand(70000, 64), operand(32000, 64, 0.05)
+    y = float8.linear(ctx, many, w, torch.empty(70000, 32000, device="cuda", dtype=torch.bfloat16))
+    want, magnitudes = wide_product(float8.Float8Rows(many.values[-200:], many.scales[-200:]), w)
+    assert torch.all((y[-200:].double() - want).abs() <= sum_off(64, magnitudes, torch.bfloat16) + half_step(torch.bfloat16) * 1.01 * want.abs())
+    del y
+    # Rows that far apart, in the form that reads them without tensor maps.
+    apart = torch.zeros(20 << 28, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn).view(20, 1 << 28)
+    spread = float8.Float8Rows(apart[:, :64], w.scales[:20].clone())
+    spread.values.copy_(w.values[:20])
+    got = float8.linear(ctx, few_rows := operand(2, 64), spread, torch.empty(2, 20, device="cuda"))
+    want, magnitudes = wide_product(few_rows, float8.Float8Rows(w.values[:20], w.scales[:20]))
+    assert torch.all((got.double() - want).abs() <= sum_off(64, magnitudes, torch.float32) + half_step(torch.float32) * 1.01 * want.abs())
+
+
 # --- refusals, without a GPU ----------------------------------------------------------------------
 
 
