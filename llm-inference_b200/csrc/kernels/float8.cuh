@@ -5,8 +5,10 @@
 //   y[m][n] = (sum_k x[m][k] w[n][k]) * xs[m] * ws[n].
 // A product of two e4m3 numbers has 8 bits, so every product is exact; sums are 32-bit. `tcgen05.mma` drops the bits below the last when it
 // adds (toward zero). Measured, a chain of n additions (32 k each) makes a sum of numbers of both signs smaller by 1.6e-9 n of itself, of one sign by
-// 1.5e-8 n: 5e-7 and 4.3e-6 for n = 296. Where outputs are 32-bit the chains are therefore cut after 64 additions (kChainBlocks) and
-// the pieces added in registers with ordinary rounding; a bfloat16 output's own rounding (2^-9) is hundreds of times what an uncut chain loses.
+// 1.5e-8 n: 5e-7 and 4.3e-6 for n = 296. Where outputs are 32-bit the chains are therefore cut after 320 additions at most (kChainBlocks: K of
+// 10,240, 5e-7 of a sum) and the pieces added in registers with ordinary rounding. More cuts cost more than they give: reading the sums takes the
+// products' time in TMEM, about a microsecond (2,048 x 5,120 x 5,120 into a 32-bit stream: cut after 64 additions 64 us, after 128 60, uncut
+// 52). A bfloat16 output's own rounding (2^-9) is hundreds of times what an uncut chain loses.
 #pragma once
 
 #include <cuda.h>
@@ -21,7 +23,7 @@ constexpr float kSmallestScale = 1.17549435e-38f;  // 2^-126: a row of zeros has
 constexpr int kRowsW = 128;                   // rows of W a block holds: TMEM lanes
 constexpr int kBlockK = 128;                  // k per stage: 128 bytes, one swizzle row
 constexpr int kMmaK = 32;
-constexpr int kChainBlocks = 16;              // 32-bit outputs: k-blocks a chain runs over (64 additions)
+constexpr int kChainBlocks = 80;              // 32-bit outputs: k-blocks a chain runs over at most (320 additions)
 constexpr long long kWaitCycles = 4000000000LL;  // about two seconds
 constexpr int ERRBIT_TIMEOUT = 8;
 
@@ -128,6 +130,7 @@ class WayOut {
     const int m = m0 + (lane >> 3);  // this lane's tokens: m, m + 4 of each eight
     to_ = static_cast<T*>(e.out) + m * e.out_stride + (KIND == GATED ? n_ >> 1 : n_);
     from_ = e.residual != nullptr ? e.residual + m * e.residual_stride + n_ : nullptr;
+    ask();
   }
 
   // The next eight tokens; `v`: sums without scales, `xs`: the tokens' scales (16-byte aligned).
@@ -135,16 +138,11 @@ class WayOut {
     const int lane = threadIdx.x & 31;
     const int left = e_.M - m_;
     const bool whole = whole_ && left >= 8;
-    float4 r[2];
+    const float4 r[2] = {residual_[0], residual_[1]};
+    m_ += apart_;
     if (KIND != GATED && e_.residual != nullptr) {
-      if (whole) {
-        r[0] = *reinterpret_cast<const float4*>(from_);
-        r[1] = *reinterpret_cast<const float4*>(from_ + 4 * e_.residual_stride);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 2; ++q) r[q] = q * 4 + (lane >> 3) < left ? residual_quad(e_, m_ + q * 4 + (lane >> 3), n_) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
       from_ += apart_ * e_.residual_stride;
+      ask();
     }
     const float2 ws = make_float2(ws_, ws_), b = make_float2(b_, b_);
 #pragma unroll
@@ -181,11 +179,24 @@ class WayOut {
         if (q * 4 + (lane >> 3) < left) store_some<KIND, T>(to_ + q * 4 * e_.out_stride, n_, e_.N, q == 0 ? mine[0] : mine[1], e_.activation);
     }
     to_ += apart_ * e_.out_stride;
-    m_ += apart_;
     __syncwarp();
   }
 
  private:
+  // The residual's numbers for the next eight tokens, before anything waits for them.
+  __device__ __forceinline__ void ask() {
+    if (KIND == GATED || e_.residual == nullptr) return;
+    const int lane = threadIdx.x & 31, left = e_.M - m_;
+    if (whole_ && left >= 8) {
+      residual_[0] = *reinterpret_cast<const float4*>(from_);
+      residual_[1] = *reinterpret_cast<const float4*>(from_ + 4 * e_.residual_stride);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        residual_[q] = q * 4 + (lane >> 3) < left ? residual_quad(e_, m_ + q * 4 + (lane >> 3), n_) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+
   const Epilogue& e_;
   float* stage_;
   int apart_;
@@ -194,6 +205,7 @@ class WayOut {
   bool whole_;
   T* to_;
   const float* from_;
+  float4 residual_[2];
 };
 
 // --- shared memory, TMA, tcgen05 -------------------------------------------------------------------

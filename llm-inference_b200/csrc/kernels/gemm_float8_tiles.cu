@@ -212,6 +212,10 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
       // The tile's token scales, for all warps; the copy of two tiles ago is read by nobody any more (a warp meets the others once a tile).
       if (tid < p.tile) x_scales[turn][tid] = m0 + tid < p.e.M ? p.e.x_scale[m0 + tid] : 0.f;
       const float* xs = x_scales[turn] + side * width;
+      // The residual's lines of the tile, a token each: they come from memory while the products run.
+      if (KIND != GATED && p.e.residual != nullptr && n0 < p.e.N)
+        for (int i = lane; i < width; i += 32)
+          if (m0 + side * width + i < p.e.M) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.e.residual + (m0 + side * width + i) * p.e.residual_stride + n0));
       // Waits for a tile's (or a chain's) sums and says where in TMEM they are.
       auto sums_of = [&](int which) {
         alive = alive && mbar_wait(&sums_full[which & 1], (which >> 1) & 1);
@@ -295,7 +299,7 @@ float tiles_time(const Product& p, int tile) {
   const int k_blocks = (p.K + kBlockK - 1) / kBlockK, clusters = b200_sm_count_host() / 2;
   const int64_t tiles = static_cast<int64_t>((p.e.M + tile - 1) / tile) * ((p.e.N + kPairRows - 1) / kPairRows);
   const float way_out = p.out_f32 ? 1.5f + tile * 0.0145f : 0.5f + tile * 0.0085f;
-  const float links = p.out_f32 && k_blocks > kChainBlocks ? 1.15f : 1.f;
+  const float links = p.out_f32 && k_blocks > kChainBlocks ? 1.05f : 1.f;
   const float turns = static_cast<float>((tiles + clusters - 1) / clusters) * max(k_blocks * (0.21f + 0.0004f * tile) * links, way_out);
   const float all = static_cast<float>(tiles) * k_blocks * (kPairRows + tile) * kBlockK / 8.5e6f * links;
   return 3.3f + max(turns, all) + way_out;
@@ -308,7 +312,8 @@ int launch_tiles(const Product& product, int tile, cudaStream_t stream) {
   p.err = product.err;
   p.K = product.K;
   p.tile = tile;
-  p.chain_blocks = kChainBlocks;
+  const int k_blocks = (product.K + kBlockK - 1) / kBlockK, chains = (k_blocks + kChainBlocks - 1) / kChainBlocks;
+  p.chain_blocks = (k_blocks + chains - 1) / chains;
   p.w_constant = product.w_constant;
   const int stage = kRowsW * kBlockK + ((tile / 2 * kBlockK + 1023) & ~1023);
   p.stages = min(kMaxStages, static_cast<int>(kRingBytes / stage));

@@ -172,9 +172,9 @@ def wide_product(x: float8.Float8Rows, w: float8.Float8Rows) -> tuple[torch.Tens
 
 
 def sum_off(k: int, magnitudes: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """What a sum may be off by: additions of 32 products in a chain (cut where outputs are 32-bit, at 2,048 of K at the longest), of chains and of
+    """What a sum may be off by: additions of 32 products in a chain (cut where outputs are 32-bit, at 10,240 of K), of chains and of
     cluster members (16), of an instruction's products, and four roundings of scales and bias."""
-    chain = math.ceil(k / 32) if dtype == torch.bfloat16 else min(math.ceil(k / 32), 64) + math.ceil(k / 512)
+    chain = math.ceil(k / 32) if dtype == torch.bfloat16 else min(math.ceil(k / 32), 320) + math.ceil(k / 10240)
     return magnitudes * 2.0**-23 * (chain + 16 + 16 + 4)
 
 
