@@ -99,15 +99,14 @@ def _device_index(ctx: StepContext) -> int:
 def _rows(name: str, m: Float8Rows, index: int) -> tuple[int, int, int, int, int]:
     """Checks rows in 8 bits; their address and pitch, the scales' address, rows and columns."""
     v, s = m.values, m.scales
-    shape = v.shape
-    if len(shape) == 2:
-        rows, columns = shape
+    if v.dim() == 2 and s.dim() == 1:
+        rows, columns = v.shape
         pitch, step = v.stride()
         if rows <= 1 or columns == 0:
             pitch = -(-columns // ROW_BYTES) * ROW_BYTES
         address = v.data_ptr()
         if (v.dtype is _E4M3 and (step == 1 or columns <= 1) and not (address | pitch) % ROW_BYTES and pitch >= columns and v.get_device() == index
-                and s.dtype is _F32 and s.shape == (rows,) and (rows <= 1 or s.stride(0) == 1) and s.get_device() == index and rows <= MOST and columns <= MOST):
+                and s.dtype is _F32 and s.numel() == rows and s.is_contiguous() and s.get_device() == index and rows <= MOST and columns <= MOST):
             return address, pitch, s.data_ptr(), rows, columns
     raise KernelError(f"float8: {name} must be e4m3 [rows, columns] whose rows are contiguous on 16-byte boundaries, with float32 [rows] scales, at most 2**30 of each, on "
                       f"{_device_name(index)}; got {v.dtype} {list(v.shape)} (strides {list(v.stride())}, {v.device}) and {s.dtype} {list(s.shape)} ({s.device})")
@@ -127,7 +126,7 @@ def _matrix(name: str, t: torch.Tensor, rows: int, columns: int, dtypes: dict[to
 
 
 def _vector(name: str, t: torch.Tensor, count: int, index: int) -> int:
-    if t.dtype is _F32 and t.shape == (count,) and (count <= 1 or t.stride(0) == 1) and t.get_device() == index:
+    if t.dtype is _F32 and t.dim() == 1 and t.numel() == count and t.is_contiguous() and t.get_device() == index:
         return t.data_ptr()
     raise KernelError(f"float8: {name} must be float32 [{count}] on {_device_name(index)}; got {t.dtype} {list(t.shape)} ({t.device})")
 
