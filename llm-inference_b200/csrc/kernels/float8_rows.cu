@@ -13,7 +13,8 @@
 // Memory bound. A row's threads each hold a few groups of 16 bytes (of single numbers where a row's length, stride or base does not allow that), all
 // asked for before the first is used. A block takes as many rows as fit its threads, so short rows do not leave lanes idle. Rows too long for
 // the registers are read twice, the second time out of L2. Of what memory takes at its copy rate: 8,192 rows of 3,584 with a bfloat16 branch output
-// 50.6 us of 49.3, 2,048 of 5,120 20.5 of 17.6.
+// 50.6 us of 49.3, 2,048 of 5,120 20.4 of 17.6; 2,048 rows of 18,944 bfloat16 to 8 bits 20.9 of 17.8 (24.9 with 73 registers a thread and two blocks an
+// SM in place of 64 and three: instructions, 80 for eight numbers, then stand in the way).
 #include "float8.cuh"
 #include "packs.cuh"
 
@@ -146,7 +147,7 @@ struct RowScale {
 
 // W: numbers a group; ITEMS: groups a thread holds (0: the row is read twice instead); THREADS: of a block at most.
 template <typename T, int W, int ITEMS, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 2 : 1)
 float8_quantize_kernel(const RowsParams p) {
   __shared__ float scratch[32];
   const int in_block = blockDim.x / p.row_threads;
