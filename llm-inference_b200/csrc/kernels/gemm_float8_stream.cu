@@ -69,25 +69,34 @@ __device__ __forceinline__ void copy_to_peer(float* dst, const float* src, uint3
 }
 
 // What one member finishes: `rows` rows of W from n0 on, the members' partial sums ([members][tokens][slice]) added in member order; `scales` and
-// `bias` are those rows'. An item is four neighbouring rows of one token; a thread takes kItems of them at a time.
-template <int KIND, typename T>
+// `bias` are those rows'. An item is four neighbouring rows of one token; a thread takes kItems of them at a time, and asks for the next ones'
+// residual before it adds (the first ones' before the partial sums have come: `wait` is called then, by every thread).
+template <int KIND, typename T, typename Wait>
 __device__ __forceinline__ void finish_slice(const Epilogue& e, const float* inbox, const float* x_scales, const float* scales, const float* bias, int m0, int tokens,
-                                             int n0, int rows, int slice, int members, int tid) {
+                                             int n0, int rows, int slice, int members, int tid, Wait wait) {
   constexpr int kItems = 2, kFinishThreads = kSumWarps * 32;
-  const int quads = (min(rows, e.N - n0) + 3) / 4;  // with rows of W left
+  const int quads = max(0, (min(rows, e.N - n0) + 3) / 4);  // with rows of W left
   const int total = quads * tokens, plane = tokens * slice;
-  for (int base = tid; base < total; base += kFinishThreads * kItems) {
-    int m[kItems], j[kItems];
-    float4 sum[kItems], r[kItems];
+  int m[kItems], j[kItems];
+  float4 r[kItems];
+  auto ask = [&](int base) {
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
-      const int item = min(base + u * kFinishThreads, total - 1);
+      const int item = base + u * kFinishThreads;
+      m[u] = j[u] = 0;
+      r[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (item >= total) continue;
       m[u] = item / quads;
       j[u] = 4 * (item - m[u] * quads);
-      r[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (KIND != GATED && e.residual != nullptr && base + u * kFinishThreads < total) r[u] = residual_quad(e, m0 + m[u], n0 + j[u]);
-      sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (KIND != GATED && e.residual != nullptr) r[u] = residual_quad(e, m0 + m[u], n0 + j[u]);
     }
+  };
+  ask(tid);
+  wait();
+  for (int base = tid; base < total; base += kFinishThreads * kItems) {
+    float4 sum[kItems];
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) sum[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int member = 0; member < members; ++member) {
 #pragma unroll
       for (int u = 0; u < kItems; ++u) sum[u] = add_each(sum[u], *reinterpret_cast<const float4*>(inbox + member * plane + m[u] * slice + j[u]));
@@ -104,6 +113,7 @@ __device__ __forceinline__ void finish_slice(const Epilogue& e, const float* inb
       if (e.vector && n + 3 < e.N) store_whole<KIND, T>(to, v, e.activation);
       else store_some<KIND, T>(to, n, e.N, v, e.activation);
     }
+    ask(base + kFinishThreads * kItems);
   }
 }
 
@@ -158,29 +168,31 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     mbar_init(&inbox_bar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     // The thread that made the barriers also loads: the first weights are on their way before the block has met.
-    if (!p.w_constant) wait_for_predecessor();
-    for (int i = 0; i < first; ++i) {
-      mbar_expect_tx(&full_bar[i], w_bytes + x_bytes);
-      load_w(i);
-    }
-    wait_for_predecessor();
-    for (int i = 0; i < first; ++i) load_x(i);
+    if (p.w_constant)
+      for (int i = 0; i < first; ++i) {
+        mbar_expect_tx(&full_bar[i], w_bytes + x_bytes);
+        load_w(i);
+      }
   }
   if constexpr (CLUSTERED) {
     __syncwarp();
     cluster_arrive();  // this block's barriers are there
   }
-  wait_for_predecessor();
-  const int slice = CLUSTERED ? slice_rows(members) : 0;
-  const int mine = rank * slice, rows = max(0, min(kRowsW - mine, slice));  // the rows this member finishes, from n0 + mine on
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  let_successor_start();
   const uint32_t tmem_base = tmem_base_shared;
 
   if (warp == 0) {
     if (lane == 0) {
+      wait_for_predecessor();
+      for (int i = 0; i < first; ++i) {
+        if (!p.w_constant) {
+          mbar_expect_tx(&full_bar[i], w_bytes + x_bytes);
+          load_w(i);
+        }
+        load_x(i);
+      }
       int sent = first;
       for (; sent < num_kb; ++sent) {
         const int s = sent % stages;
@@ -196,6 +208,7 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     }
   } else if (warp == 1) {
     // The whole warp walks the loop and one elected lane issues, so that descriptors stay in uniform registers.
+    wait_for_predecessor();  // its limit does not run while the kernel in front does
     const bool leader = elect_one();
     const uint32_t idesc = instr_desc(kRowsW, p.tile);
     const uint64_t a_first = smem_desc(smem_addr(tiles)), b_first = smem_desc(smem_addr(tiles) + w_bytes);
@@ -228,6 +241,8 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
   const int side = (warp - 2) >> 2;
   const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
   const int tid = threadIdx.x - 64;  // among the warps that finish
+  wait_for_predecessor();
+  let_successor_start();
   if constexpr (!CLUSTERED) {
     if (warp >= 2) {
       WayOut<KIND, T> way(p.e, m0 + side * 8, n0 + quarter * 32, rows_out + (warp - 2) * kStageFloats, 16);
@@ -244,6 +259,8 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
     }
   } else {
     cluster_wait();  // the other members' barriers are there
+    const int slice = slice_rows(members);
+    const int mine = rank * slice, rows = max(0, min(kRowsW - mine, slice));  // the rows this member finishes, from n0 + mine on
     float* outbox = reinterpret_cast<float*>(tiles);  // [owners][tokens][slice], where the ring was
     float* inbox = reinterpret_cast<float*>(tiles + p.inbox_at);  // [members][tokens][slice]
     const int plane = tokens * slice;
@@ -277,11 +294,16 @@ float8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_con
       if (tid == 0 && rows > 0) mbar_expect_tx(&inbox_bar, members * bytes);
       if (tid < members && tid * slice < kRowsW) copy_to_peer(inbox + rank * plane, outbox + tid * plane, bytes, &inbox_bar, tid);  // a thread per owner
     }
-    __syncwarp();
-    if (rows > 0 && !mbar_wait(&inbox_bar, 0) && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
-    __syncwarp();
-    cluster_arrive_relaxed();  // what was sent here has come
-    if (warp >= 2) finish_slice<KIND, T>(p.e, inbox, x_scales, rows_out, rows_out + kRowsW, m0, tokens, n0 + mine, rows, slice, members, tid);
+    auto inbox_filled = [&] {
+      __syncwarp();
+      if (rows > 0 && !mbar_wait(&inbox_bar, 0) && lane == 0) atomicOr(p.err, ERRBIT_TIMEOUT);
+      __syncwarp();
+      cluster_arrive_relaxed();  // what was sent here has come
+    };
+    if (warp >= 2)
+      finish_slice<KIND, T>(p.e, inbox, x_scales, rows_out, rows_out + kRowsW, m0, tokens, n0 + mine, rows, slice, members, tid, inbox_filled);
+    else
+      inbox_filled();
     __syncwarp();
     cluster_wait();  // what was sent from here has been read
   }
