@@ -72,7 +72,8 @@ B200_API int b200_float8_linear(const Float8Linear* c, cudaStream_t stream) {
   using namespace float8;
   if (c->M == 0 || c->N == 0) return 0;
   constexpr int64_t kMost = int64_t(1) << 30;  // counts and coordinates are 32-bit
-  B200_REQUIRE(c->M > 0 && c->N > 0 && c->K > 0 && c->M <= kMost && c->N <= kMost && c->K <= kMost, "float8 product: bad sizes");
+  constexpr int64_t kMostK = int64_t(1) << 28;  // a tile's products then take half a second: no wait inside a kernel runs out
+  B200_REQUIRE(c->M > 0 && c->N > 0 && c->K > 0 && c->M <= kMost && c->N <= kMost && c->K <= kMostK, "float8 product: rows, features and inner size are at most 2^30, 2^30 and 2^28");
   Product p;
   p.x = c->x, p.w = c->w, p.x_stride = c->x_pitch, p.w_stride = c->w_pitch, p.K = static_cast<int>(c->K);
   p.kind = static_cast<int>(c->kind), p.out_f32 = c->out_dtype == DTYPE_F32, p.w_constant = c->w_constant != 0, p.err = c->err;

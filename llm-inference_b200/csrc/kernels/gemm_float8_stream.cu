@@ -8,7 +8,7 @@
 // order, so a sum does not depend on timing. A block puts its sums where its ring was, one bulk copy per owner takes them to an inbox behind the
 // owner's ring, and the owner waits for the bytes: nobody waits for a member that has nothing to do with its rows, and the cluster meets only to
 // know that barriers are there and, on leaving, that copies have been read. (64 tokens of 4,608 x 3,584: 11.1 us with the cluster meeting
-// three times and single stores into neighbours' memory, 8.0 so.)
+// three times and single stores into neighbours' memory, 7.8 so.)
 //
 // 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as TMEM goes, added up as they are read.
 //

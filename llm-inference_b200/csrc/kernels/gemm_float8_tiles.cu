@@ -12,7 +12,8 @@
 //
 // Tiles are taken in strips of a few token tiles across all rows of W, so that at any time the clusters share a few rows of both operands in L2.
 // TMEM, all of it, is taken before the kernel in front has ended: shared memory leaves no room for a block of it that still wants some. Every wait is bounded: a role that
-// gives up sets the timeout bit and leaves its loop; copies in flight are waited for, and both blocks meet before either leaves.
+// gives up sets the timeout bit and leaves its loop; copies in flight are waited for, and both blocks meet before either leaves. (Asking for the first
+// tile's weights before the kernel in front has ended gains nothing here: 2,048 tokens of 4,608 x 3,584 behind a norm 34.0 us with it, 33.7 without.)
 #include "float8.cuh"
 
 namespace float8 {
@@ -33,7 +34,6 @@ struct TileParams {
   int stages;
   int tile;          // tokens
   int chain_blocks;  // k-blocks between two readings of the sums
-  int w_constant;
 };
 
 __device__ __forceinline__ uint32_t of_leader(const void* p) { return peer_address(p, 0); }
@@ -126,7 +126,8 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   if (warp == 0) {
     if (lane == 0) {
       const uint32_t leader_full = of_leader(full_bar);
-      int s = 0, phase = 0, sent = 0;
+      int s = 0, phase = 0;
+      int64_t sent = 0;
       bool alive = true;
       for (int at = cluster; at < total && alive; at += clusters) {
         int tm, tn;
@@ -152,7 +153,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           if (++s == stages) s = 0, phase ^= 1;
         }
       } else if (rank == 0) {  // both blocks' copies in flight
-        for (int i = max(0, sent - stages); i < sent; ++i) mbar_wait(&full_bar[i % stages], (i / stages) & 1);
+        for (int64_t i = max(int64_t(0), sent - stages); i < sent; ++i) mbar_wait(&full_bar[i % stages], (i / stages) & 1);
       }
     }
   } else if (warp == 1) {
@@ -314,7 +315,6 @@ int launch_tiles(const Product& product, int tile, cudaStream_t stream) {
   p.tile = tile;
   const int k_blocks = (product.K + kBlockK - 1) / kBlockK, chains = (k_blocks + kChainBlocks - 1) / kChainBlocks;
   p.chain_blocks = (k_blocks + chains - 1) / chains;
-  p.w_constant = product.w_constant;
   const int stage = kRowsW * kBlockK + ((tile / 2 * kBlockK + 1023) & ~1023);
   p.stages = min(kMaxStages, static_cast<int>(kRingBytes / stage));
   CUtensorMap w_map, x_map;

@@ -205,7 +205,7 @@ def linear(ctx: StepContext, x: Float8Rows, weight: Float8Rows, out: torch.Tenso
            residual: torch.Tensor | None = None) -> torch.Tensor:
     """``out = act(x @ weight.T + bias) + residual`` in one kernel; ``weight`` is ``[out_features, in_features]``, ``out`` bfloat16 or float32 with
     contiguous rows, ``bias`` float32, ``activation`` None, ``"silu"``, ``"gelu"`` (tanh form) or ``"squared_relu"``, ``residual`` float32 (it may be
-    ``out`` itself). Sums are 32-bit and rounded once on the way out."""
+    ``out`` itself). Sums are 32-bit and rounded once on the way out. The inner size is at most 2**28."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise KernelError(f"float8: no activation {activation!r} (there are {', '.join(str(a) for a in ACTIVATIONS)})")
