@@ -111,36 +111,39 @@ __device__ __forceinline__ float2 fma_2(float2 a, float2 b, float2 c) {
 // A warp's way out of TMEM: 32 neighbouring rows of W, one a lane (n0: lane 0's, a multiple of 32), for tokens m0, m0 + 1, ..., eight at a time. The
 // numbers pass through `stage`, 1 KB of shared memory of the warp's own, so that a lane goes on with four neighbouring rows of one token: a
 // quarter of the stores, addresses and conditions, and gates beside their up values. (Neighbours that trade numbers by shuffles took 13
-// instructions an output and 3.6 us for the 128 x 256 sums of an SM, eight warps; this takes under five.) The whole warp calls this.
+// instructions an output and 3.6 us for the 128 x 256 sums of an SM, eight warps; this takes under five.) Where rows of the output start anywhere, and at its
+// edges, each lane stores its own row's numbers one by one, 32 neighbours of an output row a warp (774 tokens of 27,055 x 5,056 into 32 bits 107 us; with quads
+// stored one by one 123). The whole warp calls this.
 constexpr int kStageFloats = 8 * 32;
 template <int KIND, typename T>
 class WayOut {
  public:
   // apart: tokens from one eight to the next.
-  __device__ __forceinline__ WayOut(const Epilogue& e, int m0, int n0, float* stage, int apart = 8) : e_(e), stage_(stage), apart_(apart) {
+  __device__ __forceinline__ WayOut(const Epilogue& e, int m0, int n0, float* stage, int apart = 8) : e_(e), stage_(stage), apart_(apart), m_(m0), n0_(n0) {
     const int lane = threadIdx.x & 31;
     ws_ = b_ = 0.f;
     if (n0 + lane < e.N) {
       ws_ = e.w_scale[n0 + lane];
       if (e.bias != nullptr) b_ = e.bias[n0 + lane];
     }
-    m_ = m0;
-    n_ = n0 + (lane & 7) * 4;
     whole_ = e.vector && n0 + 31 < e.N;
-    const int m = m0 + (lane >> 3);  // this lane's tokens: m, m + 4 of each eight
-    to_ = static_cast<T*>(e.out) + m * e.out_stride + (KIND == GATED ? n_ >> 1 : n_);
-    from_ = e.residual != nullptr ? e.residual + m * e.residual_stride + n_ : nullptr;
+    const int m = m0 + (lane >> 3), n = n0 + (lane & 7) * 4;  // this lane's tokens: m, m + 4 of each eight
+    to_ = static_cast<T*>(e.out) + m * e.out_stride + (KIND == GATED ? n >> 1 : n);
+    from_ = e.residual != nullptr ? e.residual + m * e.residual_stride + n : nullptr;
     ask();
   }
 
   // The next eight tokens; `v`: sums without scales, `xs`: the tokens' scales (16-byte aligned).
   __device__ __forceinline__ void take(const float* xs, const float (&v)[8]) {
     const int lane = threadIdx.x & 31;
-    const int left = e_.M - m_;
+    const int m = m_, left = e_.M - m;
     const bool whole = whole_ && left >= 8;
-    const float4 r[2] = {residual_[0], residual_[1]};
+    const bool add = KIND != GATED && e_.residual != nullptr;
+    float r[8], y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = residual_[i];
     m_ += apart_;
-    if (KIND != GATED && e_.residual != nullptr) {
+    if (add) {
       from_ += apart_ * e_.residual_stride;
       ask();
     }
@@ -150,62 +153,70 @@ class WayOut {
       const float4 s = *reinterpret_cast<const float4*>(xs + i);
       const float2 lo = fma_2(mul_2(make_float2(v[i], v[i + 1]), make_float2(s.x, s.y)), ws, b);
       const float2 hi = fma_2(mul_2(make_float2(v[i + 2], v[i + 3]), make_float2(s.z, s.w)), ws, b);
-      stage_[i * 32 + lane] = lo.x;
-      stage_[(i + 1) * 32 + lane] = lo.y;
-      stage_[(i + 2) * 32 + lane] = hi.x;
-      stage_[(i + 3) * 32 + lane] = hi.y;
-    }
-    __syncwarp();
-    float4 mine[2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) mine[q] = *reinterpret_cast<const float4*>(stage_ + (q * 4 + (lane >> 3)) * 32 + (lane & 7) * 4);
-    if (KIND != GATED && KIND != ACTIVATED && e_.residual != nullptr) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) mine[q] = add_each(mine[q], r[q]);
-    }
-    if constexpr (KIND == ACTIVATED) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        mine[q] = activate_quad(mine[q], e_.activation);
-        if (e_.residual != nullptr) mine[q] = add_each(mine[q], r[q]);
-      }
+      y[i] = lo.x, y[i + 1] = lo.y, y[i + 2] = hi.x, y[i + 3] = hi.y;
     }
     if (whole) {
-      store_whole<KIND, T>(to_, mine[0], e_.activation);
-      store_whole<KIND, T>(to_ + 4 * e_.out_stride, mine[1], e_.activation);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) stage_[i * 32 + lane] = y[i];
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float4 mine = *reinterpret_cast<const float4*>(stage_ + (q * 4 + (lane >> 3)) * 32 + (lane & 7) * 4);
+        if constexpr (KIND == ACTIVATED) mine = activate_quad(mine, e_.activation);
+        if (add) mine = add_each(mine, make_float4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]));
+        store_whole<KIND, T>(to_ + q * 4 * e_.out_stride, mine, e_.activation);
+      }
+      __syncwarp();
     } else {
-#pragma unroll 1
-      for (int q = 0; q < 2; ++q)
-        if (q * 4 + (lane >> 3) < left) store_some<KIND, T>(to_ + q * 4 * e_.out_stride, n_, e_.N, q == 0 ? mine[0] : mine[1], e_.activation);
+      const int n = n0_ + lane;
+      if constexpr (KIND == GATED) {
+        // Neighbours trade one of two tokens: an even lane has the gate and up value of the first, the odd one beside it those of the second.
+        const bool odd = lane & 1;
+        T* to = static_cast<T*>(e_.out) + (m + odd) * e_.out_stride + (n >> 1);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float other = __shfl_xor_sync(0xffffffffu, odd ? y[i] : y[i + 1], 1);
+          const float gate = odd ? other : y[i], up = odd ? y[i + 1] : other;
+          if (n < e_.N && i + odd < left) to[i * e_.out_stride] = from_f32<T>(e_.activation == ACT_GELU ? gated_unit<true>(gate, up) : gated_unit<false>(gate, up));
+        }
+      } else {
+        T* to = static_cast<T*>(e_.out) + m * e_.out_stride + n;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (KIND == ACTIVATED) y[i] = activate(y[i], e_.activation);
+          if (n < e_.N && i < left) to[i * e_.out_stride] = from_f32<T>(add ? y[i] + r[i] : y[i]);
+        }
+      }
     }
     to_ += apart_ * e_.out_stride;
-    __syncwarp();
   }
 
  private:
-  // The residual's numbers for the next eight tokens, before anything waits for them.
+  // The residual's numbers for the next eight tokens, before anything waits for them: as this lane's quads have them, or its own row's.
   __device__ __forceinline__ void ask() {
     if (KIND == GATED || e_.residual == nullptr) return;
     const int lane = threadIdx.x & 31, left = e_.M - m_;
     if (whole_ && left >= 8) {
-      residual_[0] = *reinterpret_cast<const float4*>(from_);
-      residual_[1] = *reinterpret_cast<const float4*>(from_ + 4 * e_.residual_stride);
-    } else {
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-        residual_[q] = q * 4 + (lane >> 3) < left ? residual_quad(e_, m_ + q * 4 + (lane >> 3), n_) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < 2; ++q) {
+        const float4 f = *reinterpret_cast<const float4*>(from_ + q * 4 * e_.residual_stride);
+        residual_[4 * q] = f.x, residual_[4 * q + 1] = f.y, residual_[4 * q + 2] = f.z, residual_[4 * q + 3] = f.w;
+      }
+    } else {
+      const float* from = e_.residual + m_ * e_.residual_stride + n0_ + lane;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) residual_[i] = n0_ + lane < e_.N && i < left ? from[i * e_.residual_stride] : 0.f;
     }
   }
 
   const Epilogue& e_;
   float* stage_;
-  int apart_;
+  int apart_, m_, n0_;
   float ws_, b_;
-  int m_, n_;
   bool whole_;
   T* to_;
   const float* from_;
-  float4 residual_[2];
+  float residual_[8];
 };
 
 // --- shared memory, TMA, tcgen05 -------------------------------------------------------------------
