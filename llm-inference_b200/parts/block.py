@@ -62,6 +62,8 @@ class PreNormResidualBlock(Part):
     def forward(self, ctx: StepContext, cache: CacheView | None, x: torch.Tensor, delta, next_norm: Part | None = None):
         mixer, ff = self.mixer, self.feed_forward
         if getattr(mixer, "float8", False):
+            # The branches stay apart from the stream until the norm behind them adds them. (Their last products adding into it by themselves: steps of 64 requests
+            # of the 1.5B shape 1.74 ms against 1.68, of the 7B shape no difference; prompts lose more, see gemm_float8_tiles.cu.)
             a = mixer.forward(ctx, cache, self.mixer_norm.forward_float8(ctx, x, delta))
             return ff.forward(ctx, self.feed_forward_norm.forward_float8(ctx, x, a))
         h = self._norm(self.mixer_norm, ctx, x, delta, getattr(mixer, "takes_folded", False))

@@ -488,3 +488,25 @@ def test_refusals():
     elsewhere = SimpleNamespace(device=torch.device("cuda:0"))
     refuses("on cuda:0", lambda: float8.quantize(elsewhere, x, rows))
     refuses("on cuda:0", lambda: float8.linear(elsewhere, rows, w, out))
+
+
+@gpu
+def test_quantize_bfloat16_that_is_not_finite(lib):
+    """Two at a time: a NaN beside a number, a pair of them, infinities of both signs."""
+    torch.manual_seed(20)
+    x = torch.randn(6, 512, device="cuda").bfloat16()
+    clean = x.clone()
+    x[1, 10] = math.nan
+    x[2, 64:72] = math.nan
+    x[3, 100], x[3, 101] = -math.inf, math.inf
+    x[4, 500] = math.inf
+    out = float8.quantize(make_ctx(lib, positions=[0]), x, float8.empty_rows(6, 512, "cuda:0"))
+    q, s = out.values.float(), out.scales
+    for row, places in ((1, [10]), (2, list(range(64, 72)))):
+        others = [i for i in range(512) if i not in places]
+        assert torch.isnan(q[row, places]).all() and math.isfinite(float(s[row]))
+        check_rows(float8.Float8Rows(out.values[row : row + 1, others], s[row : row + 1]), clean[row : row + 1, others].double(), 2.0**-23, 2.0**-22)
+    for row, places in ((3, [100, 101]), (4, [500])):
+        others = [i for i in range(512) if i not in places]
+        assert torch.isnan(q[row, places]).all() and math.isinf(float(s[row])) and torch.all(q[row, others] == 0)
+    check_rows(float8.Float8Rows(out.values[[0, 5]], s[[0, 5]]), clean[[0, 5]].double(), 2.0**-23, 2.0**-22)
