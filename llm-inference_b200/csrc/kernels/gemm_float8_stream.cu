@@ -10,7 +10,8 @@
 // know that barriers are there and, on leaving, that copies have been read. (64 tokens of 4,608 x 3,584: 11.1 us with the cluster meeting
 // three times and single stores into neighbours' memory, 7.8 so.)
 //
-// 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as TMEM goes, added up as they are read.
+// 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as a block's share of TMEM goes (128 columns, 256 where
+// it has an SM to itself; the tile's tokens each), added up as they are read. Beyond that the chains are longer, evenly.
 //
 // The first stages' weights are asked for before the kernel in front has ended where the caller says that nothing still writes them. TMEM is
 // taken first thing: an SM starts no second block that takes TMEM before the first has given up the permit to (measured: with the wait for the kernel in

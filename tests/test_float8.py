@@ -510,3 +510,27 @@ def test_quantize_bfloat16_that_is_not_finite(lib):
         others = [i for i in range(512) if i not in places]
         assert torch.isnan(q[row, places]).all() and math.isinf(float(s[row])) and torch.all(q[row, others] == 0)
     check_rows(float8.Float8Rows(out.values[[0, 5]], s[[0, 5]]), clean[[0, 5]].double(), 2.0**-23, 2.0**-22)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("columns", [1001, 4096, 20000])
+def test_rmsnorm_with_a_weight_made_just_before(lib, rows, columns):
+    """The kernel in front makes the weight, and lets its successor start before it has ended: the norm has to read what it wrote."""
+    torch.manual_seed(31)
+    ctx = make_ctx(lib, positions=[0])
+    one, w = operand(1, 2048), operand(columns, 2048, 0.05)
+    first, second = float8.Float8Rows(one.values, one.scales), float8.Float8Rows(one.values, one.scales * 3)
+    x = torch.randn(rows, columns, device="cuda")
+    want = []
+    for source in (first, second):
+        weight = float8.linear(ctx, source, w, torch.empty(1, columns, device="cuda"))
+        torch.cuda.synchronize()
+        want.append(float8.rmsnorm(ctx, x, None, weight[0], 1e-6, float8.empty_rows(rows, columns, "cuda:0")))
+    torch.cuda.synchronize()
+    weight, out = torch.empty(1, columns, device="cuda"), [float8.empty_rows(rows, columns, "cuda:0") for _ in range(40)]
+    for i, o in enumerate(out):
+        float8.linear(ctx, (first, second)[i % 2], w, weight)
+        float8.rmsnorm(ctx, x, None, weight[0], 1e-6, o)
+    for i, o in enumerate(out):
+        assert torch.equal(o.values.view(torch.uint8), want[i % 2].values.view(torch.uint8)) and torch.equal(o.scales, want[i % 2].scales)
