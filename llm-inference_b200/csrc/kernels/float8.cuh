@@ -5,9 +5,9 @@
 //   y[m][n] = (sum_k x[m][k] w[n][k]) * xs[m] * ws[n].
 // A product of two e4m3 numbers has 8 bits, so every product is exact; sums are 32-bit. `tcgen05.mma` drops the bits below the last when it
 // adds (toward zero). Measured, a chain of n additions (32 k each) makes a sum of numbers of both signs smaller by 1.6e-9 n of itself, of one sign by
-// 1.5e-8 n: 5e-7 and 4.3e-6 for n = 296. Where outputs are 32-bit the chains are therefore cut after 320 additions (kChainBlocks: K of
-// 10,240, 5e-7 of a sum) and the pieces added in registers with ordinary rounding. The streaming form has a limited number of accumulators to cut
-// with: one for a cluster member at 128 tokens, two where its block has an SM to itself, more at fewer tokens; beyond that its chains are longer. More cuts cost more than they give: reading the sums takes the
+// 1.5e-8 n: 5e-7 and 4.3e-6 for n = 296. Where outputs are 32-bit the chains are therefore cut after
+// chain_limit k-blocks and the pieces added in registers with ordinary rounding: 320 additions (K of 10,240, 5e-7 of a sum), half of that under an
+// activation, since a square or a product of two sums has twice the error of one (inner size 18,944, squared: 1.2e-6 with 320, 4.9e-7 with 160, and 777 x 4,096 57.3 -> 58.9 us). More cuts cost more than they give: reading the sums takes the
 // products' time in TMEM, about a microsecond (2,048 x 5,120 x 5,120 into a 32-bit stream: cut after 64 additions 64 us, after 128 60, uncut
 // 52). A bfloat16 output's own rounding (2^-9) is hundreds of times what an uncut chain loses.
 #pragma once
@@ -24,12 +24,13 @@ constexpr float kSmallestScale = 1.17549435e-38f;  // 2^-126: a row of zeros has
 constexpr int kRowsW = 128;                   // rows of W a block holds: TMEM lanes
 constexpr int kBlockK = 128;                  // k per stage: 128 bytes, one swizzle row
 constexpr int kMmaK = 32;
-constexpr int kChainBlocks = 80;              // 32-bit outputs: k-blocks a chain runs over (320 additions), where accumulators suffice
 constexpr long long kWaitCycles = 4000000000LL;  // about two seconds
 constexpr int ERRBIT_TIMEOUT = 8;
 
 // KIND of a product's epilogue; ACTIVATED and GATED take their function from Epilogue::activation.
 enum : int { PLAIN = 0, ACTIVATED = 1, GATED = 2 };
+// 32-bit outputs: k-blocks a chain of products runs over at most.
+constexpr int chain_limit(int kind) { return kind == PLAIN ? 80 : 40; }
 enum : int { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_SQUARED_RELU = 3 };
 
 struct Epilogue {
@@ -343,6 +344,7 @@ struct Product {
 bool skinny_takes(int M, int N, int K);
 int launch_skinny(const Product& p, cudaStream_t stream);
 // csrc/kernels/gemm_float8_stream.cu: weights streamed past few tokens, K split inside clusters.
+constexpr float kNever = 1e30f;
 float stream_time(const Product& p);
 int launch_stream(const Product& p, cudaStream_t stream);
 // csrc/kernels/gemm_float8_tiles.cu: pairs of SMs on tiles of 256 rows of W by `tile` tokens (64 to 256, a multiple of 32).

@@ -37,9 +37,9 @@ int make_map(CUtensorMap* map, const void* base, int rows, int K, int64_t stride
 // of 8,192 x 2,048: 224 tokens 19.9 us, 256 21.3, 160 22.6; 2,048 of 4,608 x 3,584: 256 27.6, 224 33.7).
 static int launch_chosen(const Product& p, cudaStream_t stream) {
   if (skinny_takes(p.e.M, p.e.N, p.K)) return launch_skinny(p, stream);
-  if (p.e.M <= 16) return launch_stream(p, stream);
   int best = 0;
-  float least = p.e.M <= 512 ? stream_time(p) : 1e30f;
+  float least = p.e.M <= 512 ? stream_time(p) : kNever;
+  if (p.e.M <= 16 && least < kNever) return launch_stream(p, stream);
   for (int tile = 64; tile <= 256 && (tile == 64 || tile < p.e.M + 32); tile += 32) {
     const float time = tiles_time(p, tile);
     if (time < least) least = time, best = tile;

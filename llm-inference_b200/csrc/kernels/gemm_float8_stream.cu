@@ -10,8 +10,8 @@
 // know that barriers are there and, on leaving, that copies have been read. (64 tokens of 4,608 x 3,584: 11.1 us with the cluster meeting
 // three times and single stores into neighbours' memory, 7.8 so.)
 //
-// 32-bit outputs: chains of kChainBlocks k-blocks (float8.cuh) have an accumulator each, as far as a block's share of TMEM goes (128 columns, 256 where
-// it has an SM to itself; the tile's tokens each), added up as they are read. Beyond that the chains are longer, evenly.
+// 32-bit outputs: chains of k-blocks (chain_limit in float8.cuh) have an accumulator each, as far as a block's share of TMEM goes (128 columns, 256 where it
+// has an SM to itself; the tile's tokens each), added up as they are read. Where that is not far enough the call is the tile form's.
 //
 // The first stages' weights are asked for before the kernel in front has ended where the caller says that nothing still writes them. TMEM is
 // taken first thing: an SM starts no second block that takes TMEM before the first has given up the permit to (measured: with the wait for the kernel in
@@ -353,6 +353,7 @@ struct StreamPlan {
   int blocks, members, tiles, tile, stages, chain_blocks, tmem_cols;
   size_t smem;
   int inbox_at;
+  bool cut;  // chains are as short as the outputs want them
 };
 
 // How many clusters of `members` blocks run at once with one block an SM (clusters do not straddle GPCs); 0 if it cannot be told.
@@ -378,8 +379,8 @@ int clusters_one_per_sm(int members) {
   return clusters;
 }
 
-// `budget`: bytes of shared memory that a block means to take.
-void size_ring(StreamPlan& plan, int k_blocks, bool f32, size_t budget) {
+// `limit`: k-blocks of a chain (0: no matter how many); `budget`: bytes of shared memory that a block means to take.
+void size_ring(StreamPlan& plan, int k_blocks, int limit, size_t budget) {
   const size_t stage = kRowsW * kBlockK + ((static_cast<size_t>(plan.tile) * kBlockK + 1023) & ~size_t(1023));
   const int per_block = (k_blocks + plan.members - 1) / plan.members;
   size_t inbox = 0, outbox = 0;
@@ -394,10 +395,11 @@ void size_ring(StreamPlan& plan, int k_blocks, bool f32, size_t budget) {
   plan.inbox_at = static_cast<int>(ring);
   plan.smem = ring + inbox + 1024;
   // Accumulators: one, or one per chain where outputs are 32-bit, as many as the block's share of TMEM holds.
-  const int wanted = f32 ? (per_block + kChainBlocks - 1) / kChainBlocks : 1;
+  const int wanted = limit > 0 ? (per_block + limit - 1) / limit : 1;
   const int most = budget > 114 * 1024 ? 256 : 128;
   const int accumulators = max(1, min(wanted, most / plan.tile));
   plan.chain_blocks = (per_block + accumulators - 1) / accumulators;
+  plan.cut = accumulators == wanted;
   plan.tmem_cols = 32;
   while (plan.tmem_cols < accumulators * plan.tile) plan.tmem_cols *= 2;
   plan.smem = max(plan.smem, max(static_cast<size_t>(plan.tmem_cols) * 227 * 1024 / 512, static_cast<size_t>(48 * 1024)));  // see the head of the file
@@ -409,7 +411,7 @@ void size_ring(StreamPlan& plan, int k_blocks, bool f32, size_t budget) {
 // tokens of 17,920 x 1,536: 140 blocks 7.3 us, 280 of half the size 12.1; of 4,608 x 3,584: 108 blocks 8.4 us, 216 9.8). Up to 16 tokens
 // half again as many blocks as SMs (one of 4,608 x 3,584: 144 blocks 5.7 us, 216 6.2). All clusters should run at once: one that has to wait for a place
 // starts when the others are done, so clusters are narrowed until they do.
-StreamPlan plan_uncached(int M, int N, int K, bool f32) {
+StreamPlan plan_uncached(int M, int N, int K, int limit) {
   StreamPlan plan;
   plan.blocks = (N + kRowsW - 1) / kRowsW;
   plan.tiles = (M + kMaxTokens - 1) / kMaxTokens;
@@ -426,31 +428,33 @@ StreamPlan plan_uncached(int M, int N, int K, bool f32) {
   plan.members = max(1, min(min(kMaxMembers, k_blocks / (plan.tile > 16 ? 7 : 6)), (alone ? sms : sms + sms / 2) / columns));
   while (plan.members > 1 && !fit(plan.members, alone ? 1 : 2)) --plan.members;
   const bool one = alone || fit(plan.members, 1);
-  size_ring(plan, k_blocks, f32, (one ? (alone ? 190 : 150) : columns * plan.members <= 2 * sms ? 100 : 66) * 1024);
+  size_ring(plan, k_blocks, limit, (one ? (alone ? 190 : 150) : columns * plan.members <= 2 * sms ? 100 : 66) * 1024);
   return plan;
 }
 
-// Plans are remembered: the occupancy question costs more than a launch. A plan goes by N, K, the padded tokens and the outputs' type only.
-StreamPlan plan_stream(int M, int N, int K, bool f32) {
+// Plans are remembered: the occupancy question costs more than a launch. A plan goes by N, K, the padded tokens and the chains' limit only.
+StreamPlan plan_stream(const Product& p) {
   static std::mutex guard;
-  static std::map<std::tuple<int, int, int, bool, int>, StreamPlan> known;
+  static std::map<std::tuple<int, int, int, int, int>, StreamPlan> known;
   int device = 0;
   cudaGetDevice(&device);
-  const int rows = (M + 15) / 16 * 16;
-  const auto key = std::make_tuple(N, K, rows, f32, device);
+  const int rows = (p.e.M + 15) / 16 * 16, limit = p.out_f32 ? chain_limit(p.kind) : 0;
+  const auto key = std::make_tuple(p.e.N, p.K, rows, limit, device);
   std::lock_guard<std::mutex> lock(guard);
   const auto found = known.find(key);
   if (found != known.end()) return found->second;
   if (known.size() >= 8192) known.clear();
-  return known[key] = plan_uncached(rows, N, K, f32);
+  return known[key] = plan_uncached(rows, p.e.N, p.K, limit);
 }
 
 }  // namespace
 
 // Microseconds, roughly: a launch, bringing sums together, and the stream (a block's k-blocks one after the other, or what all of them take out of
-// L2 at 10 to 8 TB/s and out of memory at 6.5); fitted to 17 to 512 tokens of ten matrices.
+// L2 at 10 to 8 TB/s and out of memory at 6.5); fitted to 17 to 512 tokens of ten matrices. kNever where
+// 32-bit outputs would lose more than they should.
 float stream_time(const Product& p) {
-  const StreamPlan plan = plan_stream(p.e.M, p.e.N, p.K, p.out_f32 != 0);
+  const StreamPlan plan = plan_stream(p);
+  if (!plan.cut) return kNever;
   const int k_blocks = (p.K + kBlockK - 1) / kBlockK, sms = b200_sm_count_host();
   const int columns = plan.blocks * plan.tiles;
   const int turns = (columns * plan.members + sms - 1) / sms;
@@ -463,7 +467,7 @@ float stream_time(const Product& p) {
 int launch_stream(const Product& product, cudaStream_t stream) {
   const Epilogue& e = product.e;
   const bool f32 = product.out_f32 != 0;
-  const StreamPlan plan = plan_stream(e.M, e.N, product.K, f32);
+  const StreamPlan plan = plan_stream(product);
   B200_REQUIRE(plan.smem <= kMaxDynamicSmem, "float8 product: the plan wants %zu bytes of shared memory", plan.smem);
   StreamParams p;
   p.e = e;

@@ -8,7 +8,7 @@
 // sums of one tile while the next is made in the other half of TMEM. A lane has one row of W and a quarter of the tile's tokens: scales and bias of
 // the row are the lane's own; on their way out the numbers change places inside a warp (WayOut in float8.cuh).
 //
-// 32-bit outputs: after each chain of kChainBlocks k-blocks the warps add the sums to registers and the products go on in the other half.
+// 32-bit outputs: after each chain of k-blocks (chain_limit in float8.cuh) the warps add the sums to registers and the products go on in the other half.
 //
 // Tiles are taken in strips of a few token tiles across all rows of W, so that at any time the clusters share a few rows of both operands in L2.
 // TMEM, all of it, is taken before the kernel in front has ended: shared memory leaves no room for a block of it that still wants some. Every wait is bounded: a role that
@@ -300,7 +300,7 @@ float tiles_time(const Product& p, int tile) {
   const int k_blocks = (p.K + kBlockK - 1) / kBlockK, clusters = b200_sm_count_host() / 2;
   const int64_t tiles = static_cast<int64_t>((p.e.M + tile - 1) / tile) * ((p.e.N + kPairRows - 1) / kPairRows);
   const float way_out = p.out_f32 ? 1.5f + tile * 0.0145f : 0.5f + tile * 0.0085f;
-  const float links = p.out_f32 && k_blocks > kChainBlocks ? 1.05f : 1.f;
+  const float links = p.out_f32 && k_blocks > chain_limit(p.kind) ? 1.f + 4.f / chain_limit(p.kind) : 1.f;
   const float turns = static_cast<float>((tiles + clusters - 1) / clusters) * max(k_blocks * (0.21f + 0.0004f * tile) * links, way_out);
   const float all = static_cast<float>(tiles) * k_blocks * (kPairRows + tile) * kBlockK / 8.5e6f * links;
   return 3.3f + max(turns, all) + way_out;
@@ -313,7 +313,7 @@ int launch_tiles(const Product& product, int tile, cudaStream_t stream) {
   p.err = product.err;
   p.K = product.K;
   p.tile = tile;
-  const int k_blocks = (product.K + kBlockK - 1) / kBlockK, chains = (k_blocks + kChainBlocks - 1) / kChainBlocks;
+  const int k_blocks = (product.K + kBlockK - 1) / kBlockK, chains = (k_blocks + chain_limit(product.kind) - 1) / chain_limit(product.kind);
   p.chain_blocks = (k_blocks + chains - 1) / chains;
   const int stage = kRowsW * kBlockK + ((tile / 2 * kBlockK + 1023) & ~1023);
   p.stages = min(kMaxStages, static_cast<int>(kRingBytes / stage));

@@ -534,3 +534,25 @@ def test_rmsnorm_with_a_weight_made_just_before(lib, rows, columns):
         float8.rmsnorm(ctx, x, None, weight[0], 1e-6, o)
     for i, o in enumerate(out):
         assert torch.equal(o.values.view(torch.uint8), want[i % 2].values.view(torch.uint8)) and torch.equal(o.scales, want[i % 2].scales)
+
+
+@gpu
+@pytest.mark.parametrize("m", [9, 128, 500, 777])
+@pytest.mark.parametrize("kind", ["plain", "squared_relu", "gated"])
+def test_32_bit_outputs_of_long_rows(lib, kind, m):
+    """Products are added toward zero: a chain of n additions loses 1.6e-9 n of a sum of both signs. Chains end after 320 (5.1e-7), after 160 under an
+    activation (2.6e-7, which a square or a product of two sums doubles); the pieces, scales and the function are rounded as ever, each rounding 2^-24 at most, of
+    which four at their worst add 2.4e-7, twice that through a square. Sum of both: 7.5e-7, and 9.9e-7."""
+    torch.manual_seed(32)
+    n, k = 37888 if m == 128 else 4096, 18944
+    x, w = operand(m, k), operand(n, k, 0.02)
+    ctx = make_ctx(lib, positions=[0])
+    if kind == "gated":
+        out = float8.linear_gated(ctx, x, w, torch.empty(m, n // 2, device="cuda"))
+    else:
+        out = float8.linear(ctx, x, w, torch.empty(m, n, device="cuda"), activation=None if kind == "plain" else kind)
+    a = x.values.double() * x.scales.double()[:, None]
+    y = torch.cat([a @ (w.values[at : at + 4096].double() * w.scales[at : at + 4096].double()[:, None]).t() for at in range(0, n, 4096)], dim=1)
+    want = wide_activation(y[:, 0::2], "silu") * y[:, 1::2] if kind == "gated" else wide_activation(y, None if kind == "plain" else kind)
+    off = float((out.double() - want).norm() / want.norm())
+    assert off <= (7.5e-7 if kind == "plain" else 9.9e-7)
