@@ -1,12 +1,13 @@
 // Rows of numbers to rows of e4m3 with a 32-bit scale each (float8.cuh), by themselves or as the output of an RMS norm with the residual's addition.
 //
-//   quantize:  scale = max(amax |v| / 448, 2^-126),  q = e4m3(v / scale)
+//   quantize:  scale = max(amax |v| * (1 / 448), 2^-126),  q = e4m3(v / scale), each step in 32 bits
 //   rmsnorm:   s = x + delta (written out),  v = s * rsqrt(mean s^2 + eps) * w,  then the same
 //
 // One pass: a row is read once and stays in registers. The norm's 1 / rms is a factor of the whole row, so the largest |s w| is found together with the
 // sum of squares (one meeting of the row's threads, not two), the factor drops out of q = s w / (amax |s w| / 448), and only the scale
-// has it. Divisions by the scale are products with one reciprocal a row: 448 / amax is rounded once, v times it once, which moves a quotient by
-// 2^-23 of itself at most; e4m3 rounds it by 2^-4.
+// has it. The norm's divisions by the scale are products with one reciprocal a row: 448 / amax is rounded once, v times it once, which moves a quotient by
+// 2^-23 of itself at most; e4m3 rounds it by 2^-4. quantize has to be exact: quotients of bfloat16 rows often lie on the middle between two e4m3 numbers, and one that
+// is 2^-24 off goes to the other side (Quotient below).
 // quantize: NaN stays NaN in its place (the largest magnitude is taken over the others); a row with an infinity has scale infinity, its finite numbers are
 // zeros and its infinities NaN, so what is made of that row is NaN. rmsnorm: a NaN or an infinity makes the mean, and with it the row's scale, NaN. No
 // other row is touched. A sum of squares beyond 32 bits (numbers of 1e19) counts as infinite: the row becomes zeros, as in the formula in 32 bits.
@@ -14,8 +15,8 @@
 // Memory bound. A row's threads each hold a few groups of 16 bytes (of single numbers where a row's length, stride or base does not allow that), all
 // asked for before the first is used. A block takes as many rows as fit its threads, so short rows do not leave lanes idle. Rows too long for
 // the registers are read twice, the second time out of L2. Of what memory takes at its copy rate: 8,192 rows of 3,584 with a bfloat16 branch output
-// 50.6 us of 49.3, 2,048 of 5,120 20.4 of 17.6; 2,048 rows of 18,944 bfloat16 to 8 bits 20.9 of 17.8 (24.9 with 73 registers a thread and two blocks an
-// SM in place of 64 and three: instructions, 80 for eight numbers, then stand in the way).
+// 50.6 us of 49.3, 2,048 of 5,120 20.4 of 17.6; 2,048 rows of 18,944 bfloat16 to 8 bits 21.5 of 17.8 (64 registers a thread let
+// three blocks onto an SM; instructions, some 90 for eight numbers, stand in the way with two).
 #include "float8.cuh"
 #include "packs.cuh"
 
@@ -76,9 +77,10 @@ struct Raw<T, 1> {
 };
 __device__ __forceinline__ void store_f32(float* p, const float (&f)[4]) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
 __device__ __forceinline__ void store_f32(float* p, const float (&f)[1]) { *p = f[0]; }
+__device__ __forceinline__ uint32_t four(float2 lo, float2 hi) { return to_e4m3x2(lo.x, lo.y) | to_e4m3x2(hi.x, hi.y) << 16; }
 __device__ __forceinline__ uint32_t four(const float* f, float factor) {
-  const float2 both = make_float2(factor, factor), lo = mul_2(make_float2(f[0], f[1]), both), hi = mul_2(make_float2(f[2], f[3]), both);
-  return to_e4m3x2(lo.x, lo.y) | to_e4m3x2(hi.x, hi.y) << 16;
+  const float2 both = make_float2(factor, factor);
+  return four(mul_2(make_float2(f[0], f[1]), both), mul_2(make_float2(f[2], f[3]), both));
 }
 __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[8], float factor) { *reinterpret_cast<uint2*>(p) = make_uint2(four(f, factor), four(f + 4, factor)); }
 __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[4], float factor) { *reinterpret_cast<uint32_t*>(p) = four(f, factor); }
@@ -134,6 +136,33 @@ __device__ __forceinline__ void row_sum_and_largest(float& sum, float& most, flo
 
 constexpr unsigned kPrefetchBlocks = 148;  // as many as SMs
 constexpr float kSmallestAmax = kLargest * kSmallestScale;  // rows below it have the smallest scale
+constexpr float kPerLargest = 1.f / kLargest;
+
+// A row's scale and its numbers' quotients by it, as elementary operations have them: rounded to 32 bits (to nearest even) before they are rounded to e4m3.
+// 1 / scale is held in two words, 1 / scale = hi + lo but for 2^-48 of itself, and the quotient is v lo + v hi, rounded twice, the first time far below the last
+// bit. With `lo` rounded upward no quotient comes to lie on another side of a middle between two e4m3 numbers than the rounded one (or beside a middle that
+// it should be on): tried for all 2^23 mantissas of a scale and, next to each middle, 13 numbers v, whose exponents do not matter while nothing leaves the
+// range. Numbers and scale are therefore made smaller where `lo` would be too small to have all its bits. A scale of infinity has quotients 0 and, of infinities, NaN.
+// (2,048 rows of 18,944 bfloat16 numbers 21.5 us; with the product by `hi` alone 20.2.)
+struct Quotient {
+  float scale, hi, lo, down;
+  __device__ __forceinline__ explicit Quotient(float most) {
+    scale = fmaxf(most * kPerLargest, kSmallestScale);
+    down = scale > 0x1p64f ? 0x1p-64f : 1.f;  // a normal number is left of all quotients above 2^-10
+    const float by = scale * down;
+    hi = 1.f / by;
+    lo = isinf(scale) ? 0.f : __fmul_ru(fmaf(-hi, by, 1.f), hi);
+  }
+  __device__ __forceinline__ float2 two(float a, float b) const {
+    const float2 v = make_float2(a, b);
+    return fma_2(v, make_float2(hi, hi), mul_2(v, make_float2(lo, lo)));
+  }
+  __device__ __forceinline__ float one(float v) const { return fmaf(v, hi, v * lo); }
+};
+__device__ __forceinline__ uint32_t four(const float* f, const Quotient& q) { return four(q.two(f[0], f[1]), q.two(f[2], f[3])); }
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[8], const Quotient& q) { *reinterpret_cast<uint2*>(p) = make_uint2(four(f, q), four(f + 4, q)); }
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[4], const Quotient& q) { *reinterpret_cast<uint32_t*>(p) = four(f, q); }
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[1], const Quotient& q) { *p = static_cast<uint8_t>(to_e4m3x2(q.one(f[0]), 0.f)); }
 
 // The factors of a normed row: what is held (before 1 / rms), times `first`, times `second`, is the quotient by the scale. 1 / rms cancels, 448 / most alone is
 // left, unless the row is so small that a factor would not be a normal number.
@@ -179,12 +208,16 @@ float8_quantize_kernel(const RowsParams p) {
   }
   most = row_largest(most, scratch, p.row_threads);
   if (!live) return;
-  if (t == 0) p.scales[row] = most >= kSmallestAmax ? most / kLargest : kSmallestScale;
-  const float factor = most >= kSmallestAmax ? kLargest / most : 1.f / kSmallestScale;
+  const Quotient quotient(most);
+  if (t == 0) p.scales[row] = quotient.scale;
   auto put = [&](const Raw<T, W>& g, int at) {
     float f[W];
     g.widen(f);
-    store_e4m3(out + at * W, f, factor);
+    if (quotient.down != 1.f) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) f[i] *= quotient.down;
+    }
+    store_e4m3(out + at * W, f, quotient);
   };
   if constexpr (ITEMS > 0) {
 #pragma unroll

@@ -17,6 +17,7 @@ from ..csrc.library import DTYPE_CODES, KernelError
 from .context import StepContext
 
 LARGEST = 448.0  # of e4m3
+PER_LARGEST = 1.0 / LARGEST  # scales are products with it, rounded to 32 bits, on every device (the tensor library divides by a number in its own way on each)
 SMALLEST_SCALE = 2.0**-126
 ROW_BYTES = 16  # rows start on multiples of this
 MOST = 2**30  # rows, columns
@@ -67,7 +68,7 @@ def from_tensor(weight: torch.Tensor) -> Float8Rows:
     out = empty_rows(*weight.shape, weight.device)
     for at in range(0, weight.shape[0], 4096):  # bounds the 32-bit copies
         rows = weight[at : at + 4096].float()
-        scales = torch.clamp(rows.abs().amax(1) / LARGEST, min=SMALLEST_SCALE) if rows.shape[1] else torch.full_like(out.scales[at : at + 4096], SMALLEST_SCALE)
+        scales = torch.clamp(rows.abs().amax(1) * PER_LARGEST, min=SMALLEST_SCALE) if rows.shape[1] else torch.full_like(out.scales[at : at + 4096], SMALLEST_SCALE)
         out.scales[at : at + 4096] = scales
         out.values[at : at + 4096] = (rows / scales[:, None]).clamp(-LARGEST, LARGEST).to(torch.float8_e4m3fn)
     if weight.is_cuda:
@@ -151,8 +152,9 @@ def _call(ctx: StepContext, index: int, name: str, block: bytes) -> None:
 
 
 def quantize(ctx: StepContext, x: torch.Tensor, out: Float8Rows) -> Float8Rows:
-    """``out`` = the rows of ``x`` (float32 or bfloat16, rows contiguous) in 8 bits: ``scale = max(max |row| / 448, 2**-126)``, numbers over it
-    rounded to the nearest (ties to even). NaN stays in its place; a row with an infinity has scale infinity, zeros and NaN."""
+    """``out`` = the rows of ``x`` (float32 or bfloat16, rows contiguous) in 8 bits: ``scale = max(max |row| * (1 / 448), 2**-126)``, the quotients by it
+    rounded to 32 bits and those to the nearest e4m3 number (ties to even): the numbers that elementary 32-bit operations make, and :func:`from_tensor`.
+    NaN stays in its place; a row with an infinity has scale infinity, zeros and NaN."""
     index = _device_index(ctx)
     o, o_pitch, scales, rows, columns = _rows("out", out, index)
     if columns == 0:
