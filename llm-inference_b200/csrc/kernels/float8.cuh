@@ -4,12 +4,13 @@
 // row; the number at (row, k) is q * scale. A product of two such matrices has both scales in front of the sum:
 //   y[m][n] = (sum_k x[m][k] w[n][k]) * xs[m] * ws[n].
 // A product of two e4m3 numbers has 8 bits, so every product is exact; sums are 32-bit. `tcgen05.mma` drops the bits below the last when it
-// adds (toward zero). Measured, a chain of n additions (32 k each) makes a sum of numbers of both signs smaller by 1.6e-9 n of itself, of one sign by
-// 1.5e-8 n: 5e-7 and 4.3e-6 for n = 296. Where outputs are 32-bit the chains are therefore cut after
-// chain_limit k-blocks and the pieces added in registers with ordinary rounding: 320 additions (K of 10,240, 5e-7 of a sum), half of that under an
-// activation, since a square or a product of two sums has twice the error of one (inner size 18,944, squared: 1.2e-6 with 320, 4.9e-7 with 160, and 777 x 4,096 57.3 -> 58.9 us). More cuts cost more than they give: reading the sums takes the
-// products' time in TMEM, about a microsecond (2,048 x 5,120 x 5,120 into a 32-bit stream: cut after 64 additions 64 us, after 128 60, uncut
-// 52). A bfloat16 output's own rounding (2^-9) is hundreds of times what an uncut chain loses.
+// adds (toward zero), the products' too, so a sum loses the more an addition the longer its chain is. Measured, 32 k an addition: of numbers of both signs 1.6e-9 of
+// itself an addition (5e-7 in 320), of one sign 1.1e-8 in chains of 160, 1.4e-8 in 320 (4.5e-6), 3.9e-8 in 4,096 (1.6e-4), 6.8e-8 in 16,384 (1.1e-3), 1.1e-7 in 65,536
+// (7.4e-3). Chains are therefore cut after chain_limit k-blocks and the pieces added in registers with ordinary rounding. 32-bit outputs: 320 additions (K of
+// 10,240), half of that under an activation, since a square or a product of two sums has twice the error of one (inner size 18,944, squared: 1.2e-6 with
+// 320, 4.9e-7 with 160, and 777 x 4,096 57.3 -> 58.9 us). More cuts cost more than they give: reading the sums takes the products' time in TMEM, about a
+// microsecond (2,048 x 5,120 x 5,120 into a 32-bit stream: cut after 64 additions 64 us, after 128 60, uncut 52). bfloat16 outputs: 1,024 additions (K of
+// 32,768, so that a layer's products run uncut), which take less than a hundredth of what the output's own rounding does (2^-9 to 2^-8).
 #pragma once
 
 #include <cuda.h>
@@ -29,8 +30,8 @@ constexpr int ERRBIT_TIMEOUT = 8;
 
 // KIND of a product's epilogue; ACTIVATED and GATED take their function from Epilogue::activation.
 enum : int { PLAIN = 0, ACTIVATED = 1, GATED = 2 };
-// 32-bit outputs: k-blocks a chain of products runs over at most.
-constexpr int chain_limit(int kind) { return kind == PLAIN ? 80 : 40; }
+// k-blocks a chain of products runs over at most.
+constexpr int chain_limit(int kind, bool out_f32) { return !out_f32 ? 256 : kind == PLAIN ? 80 : 40; }
 enum : int { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_SQUARED_RELU = 3 };
 
 struct Epilogue {

@@ -10,7 +10,7 @@
 // know that barriers are there and, on leaving, that copies have been read. (64 tokens of 4,608 x 3,584: 11.1 us with the cluster meeting
 // three times and single stores into neighbours' memory, 7.8 so.)
 //
-// 32-bit outputs: chains of k-blocks (chain_limit in float8.cuh) have an accumulator each, as far as a block's share of TMEM goes (128 columns, 256 where it
+// Chains of k-blocks (chain_limit in float8.cuh) have an accumulator each, as far as a block's share of TMEM goes (128 columns, 256 where it
 // has an SM to itself; the tile's tokens each), added up as they are read. Where that is not far enough the call is the tile form's.
 //
 // The first stages' weights are asked for before the kernel in front has ended where the caller says that nothing still writes them. TMEM is
@@ -353,7 +353,7 @@ struct StreamPlan {
   int blocks, members, tiles, tile, stages, chain_blocks, tmem_cols;
   size_t smem;
   int inbox_at;
-  bool cut;  // chains are as short as the outputs want them
+  bool cut;  // chains are as short as they have to be
 };
 
 // How many clusters of `members` blocks run at once with one block an SM (clusters do not straddle GPCs); 0 if it cannot be told.
@@ -379,7 +379,7 @@ int clusters_one_per_sm(int members) {
   return clusters;
 }
 
-// `limit`: k-blocks of a chain (0: no matter how many); `budget`: bytes of shared memory that a block means to take.
+// `limit`: k-blocks of a chain; `budget`: bytes of shared memory that a block means to take.
 void size_ring(StreamPlan& plan, int k_blocks, int limit, size_t budget) {
   const size_t stage = kRowsW * kBlockK + ((static_cast<size_t>(plan.tile) * kBlockK + 1023) & ~size_t(1023));
   const int per_block = (k_blocks + plan.members - 1) / plan.members;
@@ -394,8 +394,8 @@ void size_ring(StreamPlan& plan, int k_blocks, int limit, size_t budget) {
   const size_t ring = max(plan.stages * stage, outbox);
   plan.inbox_at = static_cast<int>(ring);
   plan.smem = ring + inbox + 1024;
-  // Accumulators: one, or one per chain where outputs are 32-bit, as many as the block's share of TMEM holds.
-  const int wanted = limit > 0 ? (per_block + limit - 1) / limit : 1;
+  // Accumulators: one per chain, as many as the block's share of TMEM holds.
+  const int wanted = (per_block + limit - 1) / limit;
   const int most = budget > 114 * 1024 ? 256 : 128;
   const int accumulators = max(1, min(wanted, most / plan.tile));
   plan.chain_blocks = (per_block + accumulators - 1) / accumulators;
@@ -438,7 +438,7 @@ StreamPlan plan_stream(const Product& p) {
   static std::map<std::tuple<int, int, int, int, int>, StreamPlan> known;
   int device = 0;
   cudaGetDevice(&device);
-  const int rows = (p.e.M + 15) / 16 * 16, limit = p.out_f32 ? chain_limit(p.kind) : 0;
+  const int rows = (p.e.M + 15) / 16 * 16, limit = chain_limit(p.kind, p.out_f32 != 0);
   const auto key = std::make_tuple(p.e.N, p.K, rows, limit, device);
   std::lock_guard<std::mutex> lock(guard);
   const auto found = known.find(key);
@@ -451,7 +451,7 @@ StreamPlan plan_stream(const Product& p) {
 
 // Microseconds, roughly: a launch, bringing sums together, and the stream (a block's k-blocks one after the other, or what all of them take out of
 // L2 at 10 to 8 TB/s and out of memory at 6.5); fitted to 17 to 512 tokens of ten matrices. kNever where
-// 32-bit outputs would lose more than they should.
+// chains would be too long.
 float stream_time(const Product& p) {
   const StreamPlan plan = plan_stream(p);
   if (!plan.cut) return kNever;

@@ -8,7 +8,8 @@
 // sums of one tile while the next is made in the other half of TMEM. A lane has one row of W and a quarter of the tile's tokens: scales and bias of
 // the row are the lane's own; on their way out the numbers change places inside a warp (WayOut in float8.cuh).
 //
-// 32-bit outputs: after each chain of k-blocks (chain_limit in float8.cuh) the warps add the sums to registers and the products go on in the other half.
+// After each chain of k-blocks (chain_limit in float8.cuh) the warps add the sums to registers and the products go on in the other half. bfloat16 outputs have
+// a form without that, for rows of one chain.
 //
 // Tiles are taken in strips of a few token tiles across all rows of W, so that at any time the clusters share a few rows of both operands in L2.
 // TMEM, all of it, is taken before the kernel in front has ended: shared memory leaves no room for a block of it that still wants some. Every wait is bounded: a role that
@@ -74,11 +75,10 @@ __device__ __forceinline__ void locate(int at, int tiles_m, int tiles_n, int& tm
   tm = first + in - tn * height;
 }
 
-template <int KIND, typename T>
+template <int KIND, typename T, bool CHAINED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const TileParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  constexpr bool kChained = sizeof(T) == 4;
   const uint32_t w_bytes = kRowsW * kBlockK;
   const uint32_t x_bytes = static_cast<uint32_t>(p.tile / 2) * kBlockK;
   const uint32_t stage_bytes = w_bytes + ((x_bytes + 1023u) & ~1023u);
@@ -98,7 +98,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
   const int tiles_m = (p.e.M + p.tile - 1) / p.tile, tiles_n = (p.e.N + kPairRows - 1) / kPairRows;
   const int total = tiles_m * tiles_n;
   const int k_blocks = (p.K + kBlockK - 1) / kBlockK;
-  const int links = kChained ? (k_blocks + p.chain_blocks - 1) / p.chain_blocks : 1;  // readings of a tile's sums
+  const int links = CHAINED ? (k_blocks + p.chain_blocks - 1) / p.chain_blocks : 1;  // readings of a tile's sums
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -172,7 +172,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t sums = tmem_base + half * kMostTokens;
-          const int end = kChained ? min(k_blocks, kb + p.chain_blocks) : k_blocks;
+          const int end = CHAINED ? min(k_blocks, kb + p.chain_blocks) : k_blocks;
           for (const int begin = kb; kb < end; ++kb) {
             if (!mbar_wait(&full_bar[s], phase)) {
               alive = false;
@@ -237,7 +237,7 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
           way.take(xs + c, v);
         }
       };
-      if constexpr (!kChained) {
+      if constexpr (!CHAINED) {
         WayOut<KIND, T> way(p.e, m0 + side * width, n0, stage);
         asm volatile("bar.sync 1, 512;" ::: "memory");
         const uint32_t from = sums_of(item);
@@ -287,9 +287,11 @@ float8_tiles_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_cons
 
 using TileKernel = void (*)(const CUtensorMap, const CUtensorMap, const TileParams);
 
-template <typename T>
+template <typename T, bool CHAINED>
 TileKernel pick_kind(int kind) {
-  return kind == GATED ? float8_tiles_kernel<GATED, T> : kind == ACTIVATED ? float8_tiles_kernel<ACTIVATED, T> : float8_tiles_kernel<PLAIN, T>;
+  return kind == GATED       ? float8_tiles_kernel<GATED, T, CHAINED>
+         : kind == ACTIVATED ? float8_tiles_kernel<ACTIVATED, T, CHAINED>
+                             : float8_tiles_kernel<PLAIN, T, CHAINED>;
 }
 
 }  // namespace
@@ -300,7 +302,8 @@ float tiles_time(const Product& p, int tile) {
   const int k_blocks = (p.K + kBlockK - 1) / kBlockK, clusters = b200_sm_count_host() / 2;
   const int64_t tiles = static_cast<int64_t>((p.e.M + tile - 1) / tile) * ((p.e.N + kPairRows - 1) / kPairRows);
   const float way_out = p.out_f32 ? 1.5f + tile * 0.0145f : 0.5f + tile * 0.0085f;
-  const float links = p.out_f32 && k_blocks > chain_limit(p.kind) ? 1.f + 4.f / chain_limit(p.kind) : 1.f;
+  const int limit = chain_limit(p.kind, p.out_f32 != 0);
+  const float links = k_blocks > limit ? 1.f + 4.f / limit : 1.f;
   const float turns = static_cast<float>((tiles + clusters - 1) / clusters) * max(k_blocks * (0.21f + 0.0004f * tile) * links, way_out);
   const float all = static_cast<float>(tiles) * k_blocks * (kPairRows + tile) * kBlockK / 8.5e6f * links;
   return 3.3f + max(turns, all) + way_out;
@@ -313,17 +316,20 @@ int launch_tiles(const Product& product, int tile, cudaStream_t stream) {
   p.err = product.err;
   p.K = product.K;
   p.tile = tile;
-  const int k_blocks = (product.K + kBlockK - 1) / kBlockK, chains = (k_blocks + chain_limit(product.kind) - 1) / chain_limit(product.kind);
+  const int k_blocks = (product.K + kBlockK - 1) / kBlockK, limit = chain_limit(product.kind, product.out_f32 != 0), chains = (k_blocks + limit - 1) / limit;
   p.chain_blocks = (k_blocks + chains - 1) / chains;
   const int stage = kRowsW * kBlockK + ((tile / 2 * kBlockK + 1023) & ~1023);
   p.stages = min(kMaxStages, static_cast<int>(kRingBytes / stage));
   CUtensorMap w_map, x_map;
   if (make_map(&w_map, product.w, e.N, product.K, product.w_stride, kRowsW) != 0) return -1;
   if (make_map(&x_map, product.x, e.M, product.K, product.x_stride, tile / 2) != 0) return -1;
-  const TileKernel kernel = product.out_f32 ? pick_kind<float>(product.kind) : pick_kind<__nv_bfloat16>(product.kind);
+  const int form = product.out_f32 ? 0 : chains > 1 ? 1 : 2;
+  const TileKernel kernel = form == 0   ? pick_kind<float, true>(product.kind)
+                            : form == 1 ? pick_kind<__nv_bfloat16, true>(product.kind)
+                                        : pick_kind<__nv_bfloat16, false>(product.kind);
   constexpr size_t smem = kRingBytes + 1024;
-  static OncePerDevice prepared[6];
-  if (!prepared[product.kind * 2 + (product.out_f32 ? 1 : 0)](
+  static OncePerDevice prepared[9];
+  if (!prepared[product.kind * 3 + form](
           [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess; }))
     return b200_fail("float8 product: the kernel's attributes could not be set");
   const int tiles = (e.M + tile - 1) / tile * ((e.N + kPairRows - 1) / kPairRows);
