@@ -62,13 +62,15 @@ def buffer_rows(ctx: StepContext, name: str, rows: int, columns: int) -> Float8R
 
 
 def from_tensor(weight: torch.Tensor) -> Float8Rows:
-    """A weight matrix in 8 bits, laid out once, before any step: torch operations on the weight's own device, which have ended when this returns."""
+    """A weight matrix in 8 bits, laid out once, before any step: torch operations on the weight's own device, which have ended when this returns. The
+    numbers are :func:`quantize`'s, a NaN in its place too."""
     if weight.dim() != 2:
         raise KernelError(f"float8: a matrix has two dimensions, not {weight.dim()}")
     out = empty_rows(*weight.shape, weight.device)
     for at in range(0, weight.shape[0], 4096):  # bounds the 32-bit copies
         rows = weight[at : at + 4096].float()
-        scales = torch.clamp(rows.abs().amax(1) * PER_LARGEST, min=SMALLEST_SCALE) if rows.shape[1] else torch.full_like(out.scales[at : at + 4096], SMALLEST_SCALE)
+        largest = torch.nan_to_num(rows.abs(), nan=0.0, posinf=torch.inf)  # a NaN counts for nothing beside a number
+        scales = torch.clamp(largest.amax(1) * PER_LARGEST, min=SMALLEST_SCALE) if rows.shape[1] else torch.full_like(out.scales[at : at + 4096], SMALLEST_SCALE)
         out.scales[at : at + 4096] = scales
         out.values[at : at + 4096] = (rows / scales[:, None]).clamp(-LARGEST, LARGEST).to(torch.float8_e4m3fn)
     if weight.is_cuda:

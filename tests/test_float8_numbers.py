@@ -82,3 +82,20 @@ def test_quantize_beside_every_middle():
     x = torch.where(x.abs() > most, most, x)
     out = float8.quantize(make_ctx(kernels(), positions=[0]), x, float8.empty_rows(*x.shape, "cuda:0"))
     same_numbers(out, *elementary(x))
+
+
+def test_from_tensor_keeps_a_nan_in_its_place():
+    """As `quantize` does: the row's other numbers and its scale are what they would be beside a zero."""
+    torch.manual_seed(43)
+    w = torch.randn(6, 80)
+    clean = w.clone()
+    clean[1, 5] = clean[2, 3] = clean[2, 70] = 0.0
+    w[1, 5] = w[2, 3] = w[2, 70] = math.nan
+    w[3] = math.nan
+    w[4, 9], w[4, 10] = math.inf, math.nan
+    rows, beside = float8.from_tensor(w), float8.from_tensor(clean)
+    same_numbers(rows, *elementary(w))
+    assert torch.equal(rows.scales[:3], beside.scales[:3]) and torch.equal(rows.scales[5:], beside.scales[5:])
+    q = rows.values.float()
+    assert torch.isnan(q).nonzero().tolist() == [[1, 5], [2, 3], [2, 70], *([3, i] for i in range(80)), [4, 9], [4, 10]]
+    assert torch.equal(q[:3].nan_to_num(), beside.values.float()[:3]) and float(rows.scales[3]) == 2.0**-126 and math.isinf(float(rows.scales[4]))
