@@ -68,7 +68,7 @@ def from_tensor(weight: torch.Tensor) -> Float8Rows:
         raise KernelError(f"float8: a matrix has two dimensions, not {weight.dim()}")
     out = empty_rows(*weight.shape, weight.device)
     for at in range(0, weight.shape[0], 4096):  # bounds the 32-bit copies
-        rows = weight[at : at + 4096].float()
+        rows = weight[at : at + 4096].detach().float()
         largest = torch.nan_to_num(rows.abs(), nan=0.0, posinf=torch.inf)  # a NaN counts for nothing beside a number
         scales = torch.clamp(largest.amax(1) * PER_LARGEST, min=SMALLEST_SCALE) if rows.shape[1] else torch.full_like(out.scales[at : at + 4096], SMALLEST_SCALE)
         out.scales[at : at + 4096] = scales

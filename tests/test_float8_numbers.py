@@ -99,3 +99,12 @@ def test_from_tensor_keeps_a_nan_in_its_place():
     q = rows.values.float()
     assert torch.isnan(q).nonzero().tolist() == [[1, 5], [2, 3], [2, 70], *([3, i] for i in range(80)), [4, 9], [4, 10]]
     assert torch.equal(q[:3].nan_to_num(), beside.values.float()[:3]) and float(rows.scales[3]) == 2.0**-126 and math.isinf(float(rows.scales[4]))
+
+
+def test_from_tensor_of_a_parameter_has_no_gradients():
+    """Weights laid out are numbers only: no graph that holds their 32-bit copies."""
+    torch.manual_seed(44)
+    weight = torch.nn.Parameter(torch.randn(5, 40))
+    rows = float8.from_tensor(weight)
+    assert not rows.scales.requires_grad and rows.scales.grad_fn is None and not rows.values.requires_grad and rows.values.grad_fn is None
+    same_numbers(rows, *elementary(weight.detach()))
