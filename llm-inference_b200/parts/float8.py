@@ -144,6 +144,11 @@ _pack_rmsnorm = Struct("13qd").pack
 _pack_linear = Struct("19q").pack
 
 
+def _refuse_host(index: int) -> None:
+    if index < 0:
+        raise KernelError("float8: the operands lie in host memory, and there are kernels for the GPU only")
+
+
 def _call(ctx: StepContext, index: int, name: str, block: bytes) -> None:
     """Launches on the step's device, whichever is current."""
     if _current_device() == index:
@@ -162,6 +167,7 @@ def quantize(ctx: StepContext, x: torch.Tensor, out: Float8Rows) -> Float8Rows:
     if columns == 0:
         raise KernelError("float8: rows without numbers have no scale")
     x_at, x_pitch, code = _matrix("x", x, rows, columns, _BOTH, index)
+    _refuse_host(index)
     _call(ctx, index, "b200_float8_quantize", _pack_quantize(x_at, code, x_pitch, o, o_pitch, scales, rows, columns))
     return out
 
@@ -180,8 +186,9 @@ def rmsnorm(ctx: StepContext, x: torch.Tensor, delta: torch.Tensor | None, weigh
         s_at, s_pitch, _ = _matrix("stream", stream, rows, columns, _ONLY_F32, index)
     else:
         s_at, s_pitch = (0, 0) if delta is None else (x_at, x_pitch)
-    _call(ctx, index, "b200_float8_rmsnorm", _pack_rmsnorm(x_at, x_pitch, d_at, code, d_pitch, _vector("the norm's weight", weight, columns, index), s_at, s_pitch,
-                                                           o, o_pitch, scales, rows, columns, eps))
+    w_at = _vector("the norm's weight", weight, columns, index)
+    _refuse_host(index)
+    _call(ctx, index, "b200_float8_rmsnorm", _pack_rmsnorm(x_at, x_pitch, d_at, code, d_pitch, w_at, s_at, s_pitch, o, o_pitch, scales, rows, columns, eps))
     return out
 
 
@@ -196,6 +203,7 @@ def _product(ctx: StepContext, x: Float8Rows, weight: Float8Rows, out: torch.Ten
     o, o_pitch, code = _matrix("out", out, m, n // 2 if kind == _GATED else n, _BOTH, index)
     b = 0 if bias is None else _vector("bias", bias, n, index)
     r, r_pitch, _ = (0, 0, 0) if residual is None else _matrix("residual", residual, m, n, _ONLY_F32, index)
+    _refuse_host(index)
     if m and n:
         _call(ctx, index, "b200_float8_linear", _pack_linear(x_at, x_pitch, x_scales, w_at, w_pitch, w_scales, weight.constant, o, code, o_pitch, b, r, r_pitch,
                                                              m, n, k, kind, activation, ctx.err.data_ptr()))
