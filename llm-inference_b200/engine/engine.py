@@ -400,6 +400,7 @@ class Engine:
             self.scheduler.cancel(request_id)
         self._ahead = None
         torch.cuda.synchronize(self.device)  # a step launched ahead may still be running
+        self.runner.close()
         self._closed = True
 
     def __enter__(self) -> "Engine":

@@ -113,6 +113,9 @@ class ModelRunner:
         if model.device is None:
             raise RuntimeError("load the model's weights before building a runner")
         self.model, self.cache = model, cache
+        self._running = getattr(model, "runners", None)  # the model's: captured graphs hold its weights' addresses
+        if self._running is not None:
+            self._running.add(self)
         self.device, self.dtype = model.device, model.dtype
         self.lib = kernels()
         self.max_batch_tokens = max_batch_tokens
@@ -172,6 +175,12 @@ class ModelRunner:
                 self._timed_steps += 1
                 self.host_seconds += time.perf_counter() - began
         return self._step(entries, check)
+
+    def close(self) -> None:
+        """No step follows: the model's weights may be laid out anew."""
+        self._graphs.clear()
+        if self._running is not None:
+            self._running.discard(self)
 
     def timing(self) -> dict[str, float]:
         """Totals over the steps run with ``step_timing``: the host's time inside `step`

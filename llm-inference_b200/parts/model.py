@@ -5,6 +5,7 @@ from __future__ import annotations
 from contextlib import contextmanager
 from dataclasses import dataclass, field
 from typing import Any
+from weakref import WeakSet
 
 import torch
 
@@ -86,6 +87,7 @@ class Model:
         self.dtype: torch.dtype | None = None
         self.device: torch.device | None = None
         self.weights: str | None = None  # "float8" after `to_float8`
+        self.runners: WeakSet = WeakSet()  # what runs its steps: their captured graphs hold the weights' addresses
         self._ids = None
         self.graph_safe = all(
             p.graph_safe for p in (self.embedding, *self.blocks, self.final_norm, self.head)
@@ -114,9 +116,11 @@ class Model:
 
     def to_float8(self) -> None:
         """Every layer's projections in e4m3 with a scale a row, laid out once from the loaded weights; embedding, norms and head stay as they are.
-        ``ValueError`` for a model that is not in bfloat16 or has a layer without such a form."""
+        ``ValueError`` for a model that is not in bfloat16, has a layer without such a form, or is run by an engine that is still open."""
         if self.weights == "float8":
             return
+        if self.runners:
+            raise ValueError("an engine that is still open runs this model: close it before the weights are laid out in 8 bits")
         if self.dtype != torch.bfloat16:
             raise ValueError(f"weights in 8 bits need a model that computes in bfloat16, not {self.dtype}")
         for index, block in enumerate(self.blocks):
