@@ -79,11 +79,6 @@ def from_tensor(weight: torch.Tensor) -> Float8Rows:
     return out
 
 
-def _need(cond: bool, message: str) -> None:
-    if not cond:
-        raise KernelError(message)
-
-
 # Operands are checked with as few trips into the tensor library as it takes: a decode step makes a hundred of these calls, and one of
 # them costs the device a few microseconds only.
 _E4M3, _F32, _BF16 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
