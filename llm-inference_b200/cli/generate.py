@@ -22,7 +22,8 @@ def add_engine_options(parser: argparse.ArgumentParser) -> None:
     parser.add_argument("--backend", choices=["auto", "cuda", "b200"], default="auto", help="kept from the reference's tools; this engine has one backend")
     parser.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     parser.add_argument("--weights", choices=["compute", "float8"], default="compute",
-                        help="'float8': the layers' projections in 8 bits (e4m3 with a scale a row), for architectures that have the form")
+                        help="'float8': the layers' products in 8 bits, their weights and what is multiplied with them (normed rows, attention outputs, gated units) "
+                             "alike: e4m3 with a scale a row; for architectures that have the form")
     parser.add_argument("--max-sequences", type=int, default=16)
     parser.add_argument("--max-model-length", type=int, default=2048)
     parser.add_argument("--kv-cache-mib", type=int, default=512)

@@ -120,7 +120,8 @@ class Engine:
         if model is None:
             if model_path is None:
                 raise ValueError("give the engine a model folder (config.json plus safetensors)")
-            # weights="float8": the layers' projections in e4m3 with a scale a row (half the bytes of a decode step's weights).
+            # weights="float8": the layers' projections in e4m3 with a scale a row (half the bytes of a decode step's weights), and with them the rows that they
+            # are multiplied with (normed rows, attention outputs, gated units).
             model = load_model(model_path, dtype, device, weights)
         elif model.device is None:
             raise ValueError("the model's weights are not loaded")

@@ -34,7 +34,8 @@ def parse_dtype(dtype: str | torch.dtype) -> torch.dtype:
 
 
 def parse_weights(weights: str | None) -> str | None:
-    """How the layers' projections are held: None in the compute dtype, ``"float8"`` in e4m3 with a scale a row."""
+    """How the layers' projections are held: None in the compute dtype, ``"float8"`` in e4m3 with a scale a row. The rows that they are multiplied with
+    (normed rows, attention outputs, gated units) are then cut to 8 bits too, in every step."""
     if weights in (None, "float8"):
         return weights
     raise ValueError(f"unknown weights {weights!r}; use None (the compute dtype) or 'float8'")
@@ -42,7 +43,8 @@ def parse_weights(weights: str | None) -> str | None:
 
 def load_model(model_path: str | Path, dtype: str | torch.dtype = "bfloat16", device: str | torch.device = "cuda:0", weights: str | None = None) -> Model:
     """Build the model that ``config.json`` names and load its safetensors weights; with ``weights="float8"`` the layers' projections are
-    then held in 8 bits (:meth:`Model.to_float8`)."""
+    then held in 8 bits (:meth:`Model.to_float8`), and the rows that they are multiplied with made so in each step. The whole model is laid out in the compute
+    dtype first, so it has to fit the device once in that."""
     compute_dtype, weights = parse_dtype(dtype), parse_weights(weights)
     folder = Path(model_path)
     if not folder.is_dir():

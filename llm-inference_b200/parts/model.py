@@ -115,7 +115,8 @@ class Model:
             self.head.share(self.embedding)
 
     def to_float8(self) -> None:
-        """Every layer's projections in e4m3 with a scale a row, laid out once from the loaded weights; embedding, norms and head stay as they are.
+        """Every layer's projections in e4m3 with a scale a row, laid out once from the loaded weights; embedding, norms and head stay as they are. Steps then
+        make the rows that go into those products in 8 bits too.
         ``ValueError`` for a model that is not in bfloat16, has a layer without such a form, or is run by an engine that is still open."""
         if self.weights == "float8":
             return
