@@ -10,7 +10,8 @@
 // is 2^-24 off goes to the other side (Quotient below).
 // quantize: NaN stays NaN in its place (the largest magnitude is taken over the others); a row with an infinity has scale infinity, its finite numbers are
 // zeros and its infinities NaN, so what is made of that row is NaN. rmsnorm: a NaN or an infinity makes the mean, and with it the row's scale, NaN. No
-// other row is touched. A sum of squares beyond 32 bits (numbers of 1e19) counts as infinite: the row becomes zeros, as in the formula in 32 bits.
+// other row is touched. s w is held in 32 bits before 1 / rms: weights for which it leaves their range while the normed number does not (below 1e-20, where eps is zero) are not
+// provided for. A sum of squares beyond 32 bits (numbers of 1e19) counts as infinite: the row becomes zeros, as in the formula in 32 bits.
 //
 // Memory bound. A row's threads each hold a few groups of 16 bytes (of single numbers where a row's length, stride or base does not allow that), all
 // asked for before the first is used. A block takes as many rows as fit its threads, so short rows do not leave lanes idle. Rows too long for
@@ -344,8 +345,8 @@ cudaError_t launch_shape(Kernel kernel, RowsParams p, const RowsShape& s, cudaSt
 }
 
 // Groups a thread: two where rows are few and all is latency (64 rows of 5,120: the norm with one group 3.1 us, with two 2.7); else four, of
-// eight bfloat16 numbers or of one number eight, so that what every thread does once a row counts less (1,777 rows of 1,001: 256 threads 5.9 us, 128 threads
-// 5.3). Longer rows are read twice (2,048 of 18,944 in 32 bits: 384 threads 39 us, 256 45).
+// eight bfloat16 numbers or of one number eight, so that what every thread does once a row counts less (the norm of 1,777 rows of 1,001 with a
+// 32-bit branch output, out of L2: 256 threads 7.6 us, 128 threads 6.9; out of memory 8.0 and 7.8). Longer rows are read twice (2,048 of 18,944 in 32 bits: 384 threads 39 us, 256 45).
 template <typename T, int W>
 cudaError_t launch_quantize(const RowsParams& p, cudaStream_t stream) {
   const bool few = p.rows < 2 * b200_sm_count_host();

@@ -169,7 +169,8 @@ def quantize(ctx: StepContext, x: torch.Tensor, out: Float8Rows) -> Float8Rows:
 
 def rmsnorm(ctx: StepContext, x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float, out: Float8Rows,
             stream: torch.Tensor | None = None) -> Float8Rows:
-    """``s = x + delta`` and ``out`` = the rows ``s * rsqrt(mean(s^2) + eps) * weight`` in 8 bits (:func:`quantize`). ``x`` is the 32-bit residual stream;
+    """``s = x + delta`` and ``out`` = the rows ``s * rsqrt(mean(s^2) + eps) * weight`` in 8 bits, nearest but for 32-bit rounding: a quotient within 2^-21 of
+    the middle between two e4m3 numbers may go to either. ``s * weight`` has to be in the range of 32 bits. ``x`` is the 32-bit residual stream;
     the sum goes to ``stream``, by default back into ``x`` (with no ``delta`` nothing is written unless ``stream`` is given)."""
     index = _device_index(ctx)
     o, o_pitch, scales, rows, columns = _rows("out", out, index)
